@@ -413,6 +413,40 @@ int32_t qm_linear_rows(qm_kv_pool* pool, const uint16_t* x, const uint16_t* weig
 int32_t qm_gate_up_swiglu_rows(qm_kv_pool* pool, const uint16_t* x, const uint16_t* gate_weight, const uint16_t* up_weight,
                                uint16_t* out, int32_t rows, int32_t hidden, int32_t intermediate, void* stream);
 
+/* ---- the same projections with 8-bit integer operands ----
+ * No counterpart in the reference (its projections, 17.cu:17646, :17691, :18020, are bf16).  Weights are int8 with one
+ * fp32 scale per output channel, activations int8 with one fp32 scale per token row; the integer sums are exact:
+ *   out[r][n] = bf16( float(sum_k x[r][k] * weight[n][k]) * x_scale[r] * weight_scale[n] + bias[n] + residual[r][n] )
+ * with one rounding at the end.  qm_quantize_rows_int8 makes both operands (a weight matrix is a matrix of rows too).
+ * Any number of rows: up to 64 go through a split-K cluster kernel, more through persistent 128-row tiles.
+ * in_features a multiple of 16, at most 65536; any out_features.  Tensors 16-byte aligned, x_scale 4-byte aligned;
+ * bias and residual may be NULL.  The pool's device must be the current device. */
+
+/* scale[r] = max_k |v[r][k]| / 127 and q[r][k] = v[r][k] / scale[r] to the nearest whole number, ties to even, where v
+ * is x [rows][dim] bf16 itself or, with norm_weight [dim], RMSNorm(x) kept in fp32:
+ * v[r][k] = x[r][k] * norm_weight[k] / sqrt(mean_k x[r][k]^2 + epsilon).  dim at most 24576, no alignment needed
+ * beyond the element's (16-byte aligned x, norm_weight and 8-byte aligned q with dim a multiple of 8 are faster).
+ * A row of zeros gets scale 0 and q 0; a row in which some x * norm_weight is not finite gets scale NaN and q 0, so that
+ * everything computed from it is NaN. */
+int32_t qm_quantize_rows_int8(const uint16_t* x, const uint16_t* norm_weight, float epsilon, int8_t* q, float* scale,
+                              int32_t rows, int32_t dim, void* stream);
+
+int32_t qm_linear_int8(qm_kv_pool* pool, const int8_t* x, const float* x_scale, const int8_t* weight,
+                       const float* weight_scale, const uint16_t* bias, const uint16_t* residual, uint16_t* out, int32_t rows,
+                       int32_t out_features, int32_t in_features, void* stream);
+
+/* The three projections of qm_qkv_linear: one launch for up to 64 rows, three for more. */
+int32_t qm_qkv_linear_int8(qm_kv_pool* pool, const int8_t* x, const float* x_scale, const int8_t* q_weight,
+                           const float* q_scale, const uint16_t* q_bias, const int8_t* k_weight, const float* k_scale,
+                           const uint16_t* k_bias, const int8_t* v_weight, const float* v_scale, const uint16_t* v_bias,
+                           uint16_t* q_out, uint16_t* k_out, uint16_t* v_out, int32_t rows, int32_t hidden, int32_t q_dim,
+                           int32_t kv_dim, void* stream);
+
+/* out[r][c] = bf16( silu(gate) * up ), gate and up in fp32 (no rounding in between). */
+int32_t qm_gate_up_swiglu_int8(qm_kv_pool* pool, const int8_t* x, const float* x_scale, const int8_t* gate_weight,
+                               const float* gate_scale, const int8_t* up_weight, const float* up_scale, uint16_t* out,
+                               int32_t rows, int32_t hidden, int32_t intermediate, void* stream);
+
 /* ---- the end of a decode step: codec-head logits -> next code, and the embedding rows of the next step ---- */
 
 #define QM_SAMPLE_REPETITION 1   /* repetition penalty 1.05 over the stream's history (17.cu:14063-14099)     */

@@ -85,6 +85,10 @@ ABI = {
     "qm_gate_up_swiglu": (c_int32, [c_void_p] * 5 + [c_int32, c_int32, c_int32, c_void_p]),
     "qm_linear_rows": (c_int32, [c_void_p] * 6 + [c_int32, c_int32, c_int32, c_void_p]),
     "qm_gate_up_swiglu_rows": (c_int32, [c_void_p] * 5 + [c_int32, c_int32, c_int32, c_void_p]),
+    "qm_quantize_rows_int8": (c_int32, [c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int32, c_int32, c_void_p]),
+    "qm_linear_int8": (c_int32, [c_void_p] * 8 + [c_int32, c_int32, c_int32, c_void_p]),
+    "qm_qkv_linear_int8": (c_int32, [c_void_p] * 15 + [c_int32, c_int32, c_int32, c_int32, c_void_p]),
+    "qm_gate_up_swiglu_int8": (c_int32, [c_void_p] * 8 + [c_int32, c_int32, c_int32, c_void_p]),
     "qm_final_head_sample": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_int32, c_int32,
                                        c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
     "qm_embedding_gather": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
@@ -155,6 +159,18 @@ def _check(code: int) -> None:
 
 def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
+
+
+def _packed(dtype, *tensors) -> None:
+    """The launchers take bare pointers: a tensor of another type or with gaps between its elements is refused here."""
+    for t in tensors:
+        if t is not None and (t.dtype != dtype or not t.is_cuda or not t.is_contiguous()):
+            raise ValueError(f"expected a contiguous CUDA tensor of {dtype}, got {t.dtype} on {t.device} with strides {t.stride()}")
+
+
+def _shaped(what: str, tensor, *shape) -> None:
+    if tensor is not None and tuple(tensor.shape) != shape:
+        raise ValueError(f"{what}: expected shape {shape}, got {tuple(tensor.shape)}")
 
 
 def _stream() -> int:
@@ -364,6 +380,87 @@ class TalkerAttention:
             out = torch.empty((x.shape[0], gate_weight.shape[0]), dtype=torch.bfloat16, device="cuda")
         _check(self.lib.qm_gate_up_swiglu_rows(self.pool, _ptr(x), _ptr(gate_weight), _ptr(up_weight), _ptr(out),
                                                x.shape[0], x.shape[1], gate_weight.shape[0], _stream()))
+        return out
+
+    def quantize_rows_int8(self, x, norm_weight=None, q=None, scale=None):
+        """int8 rows and one fp32 scale per row of x [rows][dim] bf16, after RMSNorm where a norm weight is given.  Used
+        for activations and, without a norm weight, for weight matrices."""
+        import torch
+
+        rows, dim = x.shape
+        q = torch.empty((rows, dim), dtype=torch.int8, device=x.device) if q is None else q
+        scale = torch.empty((rows,), dtype=torch.float32, device=x.device) if scale is None else scale
+        _packed(torch.bfloat16, x, norm_weight)
+        _packed(torch.int8, q)
+        _packed(torch.float32, scale)
+        _shaped("norm_weight", norm_weight, dim)
+        _shaped("q", q, rows, dim)
+        _shaped("scale", scale, rows)
+        _check(self.lib.qm_quantize_rows_int8(_ptr(x), _ptr(norm_weight), self.epsilon, _ptr(q), _ptr(scale), rows, dim, _stream()))
+        return q, scale
+
+    def linear_int8(self, x, x_scale, weight, weight_scale, bias=None, residual=None, out=None):
+        """bf16 rows from int8 rows and an int8 weight [out_features][in_features] with its scales."""
+        import torch
+
+        rows, inner = x.shape
+        outer = weight.shape[0]
+        out = torch.empty((rows, outer), dtype=torch.bfloat16, device=x.device) if out is None else out
+        _packed(torch.int8, x, weight)
+        _packed(torch.float32, x_scale, weight_scale)
+        _packed(torch.bfloat16, bias, residual, out)
+        _shaped("weight", weight, outer, inner)
+        _shaped("x_scale", x_scale, rows)
+        _shaped("weight_scale", weight_scale, outer)
+        _shaped("bias", bias, outer)
+        _shaped("residual", residual, rows, outer)
+        _shaped("out", out, rows, outer)
+        _check(self.lib.qm_linear_int8(self.pool, _ptr(x), _ptr(x_scale), _ptr(weight), _ptr(weight_scale), _ptr(bias),
+                                       _ptr(residual), _ptr(out), rows, outer, inner, _stream()))
+        return out
+
+    def qkv_linear_int8(self, x, x_scale, q_weight, q_scale, k_weight, k_scale, v_weight, v_scale, q_bias=None, k_bias=None,
+                        v_bias=None, out=None):
+        """The three projections of int8 rows; returns (q [rows][q_dim], k, v [rows][kv_dim]) in bf16."""
+        import torch
+
+        rows, inner = x.shape
+        if out is None:
+            out = tuple(torch.empty((rows, w.shape[0]), dtype=torch.bfloat16, device=x.device) for w in (q_weight, k_weight, v_weight))
+        _packed(torch.int8, x, q_weight, k_weight, v_weight)
+        _packed(torch.float32, x_scale, q_scale, k_scale, v_scale)
+        _packed(torch.bfloat16, q_bias, k_bias, v_bias, *out)
+        _shaped("x_scale", x_scale, rows)
+        for what, weight, scale, bias, o in (("q", q_weight, q_scale, q_bias, out[0]), ("k", k_weight, k_scale, k_bias, out[1]),
+                                             ("v", v_weight, v_scale, v_bias, out[2])):
+            outer = k_weight.shape[0] if what == "v" else weight.shape[0]
+            _shaped(what + " weight", weight, outer, inner)
+            _shaped(what + " scale", scale, outer)
+            _shaped(what + " bias", bias, outer)
+            _shaped(what + " output", o, rows, outer)
+        _check(self.lib.qm_qkv_linear_int8(
+            self.pool, _ptr(x), _ptr(x_scale), _ptr(q_weight), _ptr(q_scale), _ptr(q_bias), _ptr(k_weight), _ptr(k_scale),
+            _ptr(k_bias), _ptr(v_weight), _ptr(v_scale), _ptr(v_bias), _ptr(out[0]), _ptr(out[1]), _ptr(out[2]), rows, inner,
+            q_weight.shape[0], k_weight.shape[0], _stream()))
+        return out
+
+    def gate_up_swiglu_int8(self, x, x_scale, gate_weight, gate_scale, up_weight, up_scale, out=None):
+        """silu(gate) * up in bf16 from int8 rows and two int8 weights [intermediate][hidden]."""
+        import torch
+
+        rows, inner = x.shape
+        outer = gate_weight.shape[0]
+        out = torch.empty((rows, outer), dtype=torch.bfloat16, device=x.device) if out is None else out
+        _packed(torch.int8, x, gate_weight, up_weight)
+        _packed(torch.float32, x_scale, gate_scale, up_scale)
+        _packed(torch.bfloat16, out)
+        _shaped("x_scale", x_scale, rows)
+        for what, weight, scale in (("gate", gate_weight, gate_scale), ("up", up_weight, up_scale)):
+            _shaped(what + " weight", weight, outer, inner)
+            _shaped(what + " scale", scale, outer)
+        _shaped("out", out, rows, outer)
+        _check(self.lib.qm_gate_up_swiglu_int8(self.pool, _ptr(x), _ptr(x_scale), _ptr(gate_weight), _ptr(gate_scale),
+                                               _ptr(up_weight), _ptr(up_scale), _ptr(out), rows, inner, outer, _stream()))
         return out
 
     def final_head_sample(self, logits, generation_index=None, history=None, flags=0, eos_token=2150,

@@ -1,0 +1,764 @@
+// Projections with 8-bit integer operands: activations quantised per token row, weights per output channel.
+//
+//   s_x[r] = max_k |x[r][k]| / 127        q[r][k] = round(127 x[r][k] / max_k |x[r][k]|)      (ties to even)
+//   out[r][n] = (sum_k q[r][k] w[n][k]) * s_x[r] * s_w[n]  (+ bias[n]) (+ residual[r][n]), rounded to bf16 once
+//
+// The integer sums are exact (kind::i8 accumulates in 32 bits; |sum| <= 128^2 K stays below 2^31 for K up to 65 536),
+// so neither the split of K over CTAs nor the order of the chunks can change a result.  No counterpart in the
+// reference, whose projections are bf16 only (launch_linear_m1 17.cu:17646, launch_qkv_m1 :17691,
+// launch_gate_up_swiglu_m1 :18020; the calls here have their shapes).  Against those, the weights are half the bytes,
+// which is what a decode step streams, and the tensor pipe has twice the rate, which is what a prompt is bound by.
+//
+// Three kernels:
+//   qm_quantize_rows_kernel   one CTA per row; RMSNorm in front of the quantisation where a norm weight is given
+//   qm_skinny_int8_kernel     up to 64 token rows: the weight tile is the M operand, K split over a cluster
+//   qm_rows_int8_kernel       more rows: persistent 128-row tiles, two TMEM accumulators
+#include <math_constants.h>
+
+#include "qm_cluster.cuh"
+#include "qm_tcgen05.cuh"
+
+namespace {
+
+// ---- quantisation of rows -----------------------------------------------------------------------------------------
+
+constexpr int kQuantThreads = 256;
+constexpr int kQuantMaxDim = 24 * 1024;        // the row is staged in shared memory as bf16
+
+// One row.  With a norm weight the value quantised is n[k] = x[k] * w[k] / rms; the rms divides out of q (q is a ratio
+// of two such values) and enters the scale alone, so one sweep collects both the sum of squares and the largest
+// |x w|, and x w is exact in fp32 (two 8-bit significands).  A power of two keeps very large and very small rows
+// inside fp32's range.  A row with an infinity or a NaN gets scale NaN and q = 0: every output of that row is NaN.
+struct QuantRow {
+    float pre;          // exact power of two applied to the values
+    float ratio;        // 127 / (largest * pre)
+    float largest;      // largest * pre
+};
+
+__device__ __forceinline__ int quantize_value(float v, const QuantRow& r) {
+    const float scaled = v * r.pre;
+    float t = scaled * r.ratio;
+    // The product is within 2e-5 of the quotient.  Only next to a half step can that change the rounding, and there
+    // the correctly rounded quotient decides (127 * scaled is exact: at most 7 + 16 bits).
+    if (fabsf(fabsf(t - rintf(t)) - 0.5f) < 1.0e-4f) t = __fdiv_rn(127.0f * scaled, r.largest);
+    return (int)rintf(t);
+}
+
+template <bool kVector>
+__global__ void __launch_bounds__(kQuantThreads) qm_quantize_rows_kernel(const uint16_t* __restrict__ x,
+                                                                        const uint16_t* __restrict__ norm_weight,
+                                                                        float epsilon, int8_t* __restrict__ q,
+                                                                        float* __restrict__ scale, int dim) {
+    extern __shared__ uint4 row_vectors[];
+    __shared__ float warp_sum[kQuantThreads / 32], warp_max[kQuantThreads / 32];
+    __shared__ int warp_bad[kQuantThreads / 32];
+    pdl_wait();
+    pdl_trigger();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const size_t base = (size_t)blockIdx.x * dim;
+    uint16_t* staged = reinterpret_cast<uint16_t*>(row_vectors);
+    float sum = 0.0f, big = 0.0f;
+    bool bad = false;
+    auto take = [&](float v, float w) {
+        sum = fmaf(v, v, sum);
+        const float m = fabsf(v * w);
+        bad |= !(m < CUDART_INF_F);
+        big = fmaxf(big, m);
+    };
+    if (kVector) {
+        for (int v = tid; v < dim / 8; v += kQuantThreads) {
+            const uint4 raw = *reinterpret_cast<const uint4*>(x + base + 8 * v);
+            row_vectors[v] = raw;
+            uint4 wv = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);      // ones
+            if (norm_weight) wv = __ldg(reinterpret_cast<const uint4*>(norm_weight + 8 * v));
+            const uint32_t* rw = reinterpret_cast<const uint32_t*>(&raw);
+            const uint32_t* ww = reinterpret_cast<const uint32_t*>(&wv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                take(bf16_lo(rw[i]), bf16_lo(ww[i]));
+                take(bf16_hi(rw[i]), bf16_hi(ww[i]));
+            }
+        }
+    } else {
+        for (int c = tid; c < dim; c += kQuantThreads) {
+            const uint16_t raw = x[base + c];
+            staged[c] = raw;
+            take(bf16_bits_to_f32(raw), norm_weight ? bf16_bits_to_f32(norm_weight[c]) : 1.0f);
+        }
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+    }
+    bad = __any_sync(0xffffffffu, bad);
+    if (lane == 0) {
+        warp_sum[warp] = sum;
+        warp_max[warp] = big;
+        warp_bad[warp] = bad;
+    }
+    __syncthreads();
+    sum = 0.0f;
+    big = 0.0f;
+    int any_bad = 0;
+#pragma unroll
+    for (int w = 0; w < kQuantThreads / 32; ++w) {
+        sum += warp_sum[w];
+        big = fmaxf(big, warp_max[w]);
+        any_bad |= warp_bad[w];
+    }
+    QuantRow r;
+    r.pre = big > 1.0e30f ? 0x1p-64f : (big < 1.0e-30f ? 0x1p64f : 1.0f);
+    r.largest = big * r.pre;
+    const bool flat = !(big > 0.0f) || any_bad;           // nothing to quantise: every q is zero
+    r.ratio = flat ? 0.0f : 127.0f / r.largest;
+    if (tid == 0) {
+        float s = big / 127.0f;
+        if (norm_weight) s *= rsqrtf(sum / (float)dim + epsilon);
+        scale[blockIdx.x] = any_bad ? CUDART_NAN_F : s;
+    }
+    if (kVector) {
+        for (int v = tid; v < dim / 8; v += kQuantThreads) {
+            const uint4 raw = row_vectors[v];
+            uint4 wv = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+            if (norm_weight) wv = __ldg(reinterpret_cast<const uint4*>(norm_weight + 8 * v));
+            const uint32_t* rw = reinterpret_cast<const uint32_t*>(&raw);
+            const uint32_t* ww = reinterpret_cast<const uint32_t*>(&wv);
+            uint32_t packed[2] = {0u, 0u};
+            if (!flat) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int lo = quantize_value(bf16_lo(rw[i]) * bf16_lo(ww[i]), r);
+                    const int hi = quantize_value(bf16_hi(rw[i]) * bf16_hi(ww[i]), r);
+                    packed[i >> 1] |= ((uint32_t)(lo & 0xff) | ((uint32_t)(hi & 0xff) << 8)) << (16 * (i & 1));
+                }
+            }
+            *reinterpret_cast<uint2*>(q + base + 8 * v) = make_uint2(packed[0], packed[1]);
+        }
+    } else {
+        for (int c = tid; c < dim; c += kQuantThreads) {
+            const float w = norm_weight ? bf16_bits_to_f32(norm_weight[c]) : 1.0f;
+            q[base + c] = flat ? (int8_t)0 : (int8_t)quantize_value(bf16_bits_to_f32(staged[c]) * w, r);
+        }
+    }
+}
+
+// ---- shared by the two products -----------------------------------------------------------------------------------
+
+constexpr int kChunk = 128;                    // K columns (bytes) per ring stage: one 128-byte swizzle atom
+constexpr int kProductThreads = 192;           // warps 0-3 epilogue, warp 4 MMA issue, warp 5 TMA
+constexpr int kWeightRows = 128;
+
+// gate * sigmoid(gate) * up in fp32
+__device__ __forceinline__ float gated(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
+
+// The copying thread sees its last copies land (bounded) before it leaves, so that none is in flight into the shared
+// memory of a CTA that has retired after some other thread's wait gave up.
+template <typename FullBar>
+__device__ __forceinline__ void drain_ring(FullBar full_bar, int loads, int stages) {
+    bool gave_up = false;
+    for (int i = loads > stages ? loads - stages : 0; i < loads; ++i)
+        mbar_wait_bounded(full_bar(i % stages), (i / stages) & 1, gave_up);
+}
+
+struct Int8Args {
+    const float* x_scale;            // [rows]
+    const float* w_scale[3];         // [out_cols] of each weight matrix (gated: gate, up)
+    const int8_t* weight[3];
+    const uint16_t* bias[3];         // [out_cols] or null
+    const uint16_t* residual;        // [rows][out_cols] or null (one matrix only)
+    uint16_t* out[3];                // [rows][out_cols]
+    int out_cols[3];
+    int first_tile[3];               // first tile of each matrix
+    uint32_t* status;
+    int rows;
+    int k_dim;
+    int chunks;                      // ceil(k_dim / 128): the last chunk is filled up with zeros by the copy
+    int split;                       // cluster size (skinny)
+    int m_tiles, n_tiles;            // (many rows)
+};
+
+// ---- up to 64 token rows --------------------------------------------------------------------------------------------
+//
+// D^T[128 weight rows][token rows] accumulates in 16 / 32 / 64 TMEM columns; the CTAs of a cluster share a tile's K
+// range and fold their integer sums through distributed shared memory.  While the launch waits for its predecessor
+// (which writes the activations) it only asks the L2 for its weight slice: a weight matrix may be one that
+// the previous launch has just quantised, so no weight byte is read into the SM before the wait.
+template <int kMPad>
+struct SkinnySmem {
+    static constexpr int kStages = 4;
+    static constexpr int kWeightBytes = kWeightRows * kChunk;
+    static constexpr int kStageBytes = kWeightBytes + kMPad * kChunk;
+    static constexpr int kReduce = 0;                                      // int32[kMPad][128], over the spent ring
+    static constexpr int kBars = kStages * kStageBytes;                    // full[kStages], empty[kStages], acc
+    static constexpr int kTmemSlot = kBars + (2 * kStages + 1) * 8;
+    static constexpr int kTotal = kTmemSlot + 16;
+    static_assert(kMPad * kWeightRows * 4 <= kStages * kStageBytes, "the reduction buffer lies inside the ring");
+};
+
+__device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t remote_addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(remote_addr));
+    return v;
+}
+
+template <int kMPad, bool kGated>
+__global__ void __launch_bounds__(kProductThreads)
+qm_skinny_int8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap w2_map,
+                      const __grid_constant__ CUtensorMap w3_map, const __grid_constant__ CUtensorMap x_map, const Int8Args a) {
+    using L = SkinnySmem<kMPad>;
+    constexpr int kTmemCols = kMPad < 32 ? 32 : kMPad;
+    pdl_trigger();
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t raw_addr = smem_addr(smem_raw);
+    const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
+    unsigned char* smem = smem_raw + pad;
+    const uint32_t sbase = raw_addr + pad;
+    const uint32_t bar0 = sbase + L::kBars;
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (L::kStages + s); };
+    const uint32_t acc_bar = bar0 + 8u * (2 * L::kStages);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kTmemSlot);
+    int* reduce = reinterpret_cast<int*>(smem + L::kReduce);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_rank();
+    const int global_tile = blockIdx.x / a.split;
+    const int seg = kGated ? 0 : (global_tile >= a.first_tile[2] ? 2 : (global_tile >= a.first_tile[1] ? 1 : 0));
+    const int tile = global_tile - a.first_tile[seg];
+    const CUtensorMap* seg_map = seg == 0 ? &w_map : (seg == 1 ? &w2_map : &w3_map);
+    const int chunk_begin = (int)((long long)a.chunks * rank / a.split);
+    const int chunk_end = (int)((long long)a.chunks * (rank + 1) / a.split);
+    const int n_chunks = chunk_end - chunk_begin;
+
+    if (warp == 5 && lane == 0) {
+        for (int s = 0; s < L::kStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        mbar_init(acc_bar, 1);
+        fence_mbar_init();
+    }
+    if (warp == 4) {
+        tmem_alloc(smem_addr(tmem_slot), kTmemCols);
+        tmem_relinquish();
+    }
+    if (warp < 4) {
+        // one weight row's share of this CTA's K range per thread
+        const int8_t* wbase = kGated ? (tid < 64 ? a.weight[0] : a.weight[1]) : a.weight[seg];
+        const int wrow = kGated ? tile * 64 + (tid & 63) : tile * kWeightRows + tid;
+        const int k0 = chunk_begin * kChunk;
+        const int k1 = chunk_end * kChunk < a.k_dim ? chunk_end * kChunk : a.k_dim;
+        if (wrow < a.out_cols[seg] && k1 > k0)
+            bulk_prefetch_l2_hint(wbase + (size_t)wrow * a.k_dim + k0, (uint32_t)(k1 - k0), l2_policy_evict_last());
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+    bool dead = false;
+    pdl_wait();
+
+    if (warp == 5) {
+        if (lane == 0) {
+            const uint64_t weights_once = l2_policy_evict_first();
+            for (int i = 0; i < n_chunks; ++i) {
+                const int st = i % L::kStages;
+                if (!mbar_wait_bounded(empty_bar(st), ((i / L::kStages) & 1) ^ 1, dead)) atomicOr(a.status, QM_DEVSTAT_TIMEOUT);
+                const uint32_t dst = sbase + st * L::kStageBytes;
+                const int col = (chunk_begin + i) * kChunk;
+                mbar_arrive_expect_tx(full_bar(st), L::kStageBytes);
+                tma_load_2d(dst + L::kWeightBytes, &x_map, full_bar(st), col, 0);
+                if (kGated) {
+                    tma_load_2d_hint(dst, &w_map, full_bar(st), col, tile * 64, weights_once);
+                    tma_load_2d_hint(dst + L::kWeightBytes / 2, &w2_map, full_bar(st), col, tile * 64, weights_once);
+                } else {
+                    tma_load_2d_hint(dst, seg_map, full_bar(st), col, tile * kWeightRows, weights_once);
+                }
+            }
+            drain_ring(full_bar, n_chunks, L::kStages);
+        }
+        __syncwarp();
+    } else if (warp == 4) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = umma_instr_desc_s8(kWeightRows, kMPad);
+            for (int i = 0; i < n_chunks; ++i) {
+                const int st = i % L::kStages;
+                if (!mbar_wait_bounded(full_bar(st), (i / L::kStages) & 1, dead)) atomicOr(a.status, QM_DEVSTAT_TIMEOUT);
+                tc_fence_after();
+                const uint32_t wa = sbase + st * L::kStageBytes;
+                const uint32_t xa = wa + L::kWeightBytes;
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                    mma_i8_ss(tmem_base, smem_desc(wa + ks * 32, 16, 1024), smem_desc(xa + ks * 32, 16, 1024), idesc,
+                              (i > 0 || ks > 0) ? 1u : 0u);
+                tc_commit(empty_bar(st));
+            }
+            tc_commit(acc_bar);
+        }
+        __syncwarp();
+    } else {
+        if (!mbar_wait_bounded(acc_bar, 0, dead) && lane == 0) atomicOr(a.status, QM_DEVSTAT_TIMEOUT);
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + ((uint32_t)(warp * 32) << 16);
+#pragma unroll
+        for (int c = 0; c < kMPad / 16; ++c) {
+            uint32_t v[16];
+            if (n_chunks > 0) {
+                tmem_ld16(taddr + c * 16, v);
+                tmem_wait_ld();
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) reduce[(c * 16 + i) * kWeightRows + tid] = (int)v[i];
+        }
+    }
+    cluster_sync_all();
+
+    if (warp < 4) {
+        // rank r finishes the token rows r, r + split, ...; a work item is one of them x four weight rows
+        const uint32_t reduce_addr = sbase + L::kReduce;
+        constexpr int kGroups = kGated ? 16 : 32;
+        uint32_t peer[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) peer[k] = map_to_rank(reduce_addr, (uint32_t)(k < a.split ? k : 0));
+        const int owned = ((int)rank < a.rows) ? (a.rows - 1 - (int)rank) / a.split + 1 : 0;
+        const int n_cols = a.out_cols[seg];
+        for (int item = tid; item < owned * kGroups; item += 128) {
+            const int g = item % kGroups;
+            const int m = (int)rank + (item / kGroups) * a.split;
+            const uint32_t off = (uint32_t)(m * kWeightRows + 4 * g) * 4u;
+            int acc[4] = {0, 0, 0, 0}, acc2[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (k >= a.split) break;
+                const int4 p = ld_cluster_s32x4(peer[k] + off);
+                acc[0] += p.x; acc[1] += p.y; acc[2] += p.z; acc[3] += p.w;
+                if (kGated) {
+                    const int4 p2 = ld_cluster_s32x4(peer[k] + off + 64u * 4u);
+                    acc2[0] += p2.x; acc2[1] += p2.y; acc2[2] += p2.z; acc2[3] += p2.w;
+                }
+            }
+            const int col = (kGated ? tile * 64 : tile * kWeightRows) + 4 * g;
+            const size_t o = (size_t)m * n_cols + col;
+            const float sx = a.x_scale[m];
+            uint32_t bits[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                bits[i] = 0u;
+                if (col + i >= n_cols) continue;
+                float v = (float)acc[i] * sx * __ldg(a.w_scale[seg] + col + i);
+                if (kGated) {
+                    v = gated(v, (float)acc2[i] * sx * __ldg(a.w_scale[1] + col + i));
+                } else {
+                    if (a.bias[seg]) v += bf16_bits_to_f32(__ldg(a.bias[seg] + col + i));
+                    if (a.residual) v += bf16_bits_to_f32(a.residual[o + i]);
+                }
+                bits[i] = f32_to_bf16_bits(v);
+            }
+            uint16_t* dst = a.out[seg] + o;
+            if (col + 3 < n_cols && (reinterpret_cast<uintptr_t>(dst) & 7u) == 0) {
+                *reinterpret_cast<uint2*>(dst) = make_uint2(bits[0] | (bits[1] << 16), bits[2] | (bits[3] << 16));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (col + i < n_cols) dst[i] = (uint16_t)bits[i];
+            }
+        }
+    }
+
+    cluster_arrive_relaxed();        // nobody leaves while a peer may still read its shared memory
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 4) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, kTmemCols);
+    }
+    cluster_wait();
+}
+
+// ---- more token rows ------------------------------------------------------------------------------------------------
+//
+// One CTA per SM walks tiles of 128 token rows x kBN weight rows (gated: kBN / 2 gate rows and the same up rows); the
+// MMA thread fills one TMEM accumulator while the epilogue warps drain the other.  kBN = 256 has the fewest
+// operand bytes per operation; the narrower tiles are for calls whose 256-wide tiles would leave SMs without one.
+template <int kBN>
+struct RowsSmem {
+    static constexpr int kStageA = 128 * kChunk;
+    static constexpr int kStageBytes = kStageA + kBN * kChunk;
+    static constexpr int kStages = kBN == 256 ? 4 : (kBN == 128 ? 6 : 8);
+    static constexpr int kBars = kStages * kStageBytes;                    // full, empty, acc_full[2], acc_empty[2]
+    static constexpr int kTmemSlot = kBars + (2 * kStages + 4) * 8;
+    static constexpr int kTotal = kTmemSlot + 16;
+};
+
+template <int kBN, bool kGated>
+__global__ void __launch_bounds__(kProductThreads, 1)
+qm_rows_int8_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w0_map,
+                    const __grid_constant__ CUtensorMap w1_map, const Int8Args a) {
+    using L = RowsSmem<kBN>;
+    constexpr int kCols = kGated ? kBN / 2 : kBN;           // output columns per tile
+    pdl_trigger();
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t raw_addr = smem_addr(smem_raw);
+    const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
+    unsigned char* smem = smem_raw + pad;
+    const uint32_t sbase = raw_addr + pad;
+    const uint32_t bar0 = sbase + L::kBars;
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (L::kStages + s); };
+    auto acc_full = [&](int b) { return bar0 + 8u * (2 * L::kStages + b); };
+    auto acc_empty = [&](int b) { return bar0 + 8u * (2 * L::kStages + 2 + b); };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kTmemSlot);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < L::kStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(acc_full(b), 1);
+            mbar_init(acc_empty(b), 128);
+        }
+        fence_mbar_init();
+    }
+    if (warp == 4) {
+        tmem_alloc(smem_addr(tmem_slot), 2 * kBN);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+    const int total_tiles = a.m_tiles * a.n_tiles;
+    bool dead = false;
+    pdl_wait();
+
+    if (warp == 5) {
+        if (lane == 0) {
+            int it = 0;
+            for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x) {
+                const int m0 = (tile / a.n_tiles) * 128;
+                const int n0 = (tile % a.n_tiles) * kCols;
+                for (int kc = 0; kc < a.chunks; ++kc, ++it) {
+                    const int st = it % L::kStages;
+                    if (!mbar_wait_bounded(empty_bar(st), ((it / L::kStages) & 1) ^ 1, dead)) atomicOr(a.status, QM_DEVSTAT_TIMEOUT);
+                    const uint32_t dst = sbase + st * L::kStageBytes;
+                    mbar_arrive_expect_tx(full_bar(st), L::kStageBytes);
+                    tma_load_2d(dst, &x_map, full_bar(st), kc * kChunk, m0);
+                    tma_load_2d(dst + L::kStageA, &w0_map, full_bar(st), kc * kChunk, n0);
+                    if (kGated)
+                        tma_load_2d(dst + L::kStageA + kBN / 2 * kChunk, &w1_map, full_bar(st), kc * kChunk, n0);
+                    else
+                        tma_load_2d(dst + L::kStageA + kBN / 2 * kChunk, &w0_map, full_bar(st), kc * kChunk, n0 + kBN / 2);
+                }
+            }
+            drain_ring(full_bar, it, L::kStages);
+        }
+        __syncwarp();
+    } else if (warp == 4) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = umma_instr_desc_s8(128, kBN);
+            int it = 0, local = 0;
+            for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++local) {
+                const int buf = local & 1;
+                if (!mbar_wait_bounded(acc_empty(buf), ((local >> 1) & 1) ^ 1, dead)) atomicOr(a.status, QM_DEVSTAT_TIMEOUT);
+                tc_fence_after();
+                uint32_t seen = mbar_probe(full_bar(it % L::kStages), (it / L::kStages) & 1);
+                for (int kc = 0; kc < a.chunks; ++kc, ++it) {
+                    const int st = it % L::kStages;
+                    if (!mbar_wait_probed(seen, full_bar(st), (it / L::kStages) & 1, dead)) atomicOr(a.status, QM_DEVSTAT_TIMEOUT);
+                    seen = kc + 1 < a.chunks ? mbar_probe(full_bar((it + 1) % L::kStages), ((it + 1) / L::kStages) & 1) : 0u;
+                    tc_fence_after();
+                    const uint32_t xa = sbase + st * L::kStageBytes;
+                    const uint32_t wa = xa + L::kStageA;
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+                        mma_i8_ss(tmem_base + buf * kBN, smem_desc(xa + ks * 32, 16, 1024), smem_desc(wa + ks * 32, 16, 1024), idesc,
+                                  (kc > 0 || ks > 0) ? 1u : 0u);
+                    tc_commit(empty_bar(st));
+                }
+                tc_commit(acc_full(buf));
+            }
+        }
+        __syncwarp();
+    } else {
+        const int row_in_tile = warp * 32 + lane;
+        const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+        const int n_cols = a.out_cols[0];
+        const bool wide = (n_cols & 7) == 0;               // every 8-column piece of a row is then 16-byte aligned
+        int local = 0;
+        for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++local) {
+            const int buf = local & 1;
+            const int n0 = (tile % a.n_tiles) * kCols;
+            const int row = (tile / a.n_tiles) * 128 + row_in_tile;
+            if (!mbar_wait_bounded(acc_full(buf), (local >> 1) & 1, dead) && lane == 0) atomicOr(a.status, QM_DEVSTAT_TIMEOUT);
+            tc_fence_after();
+            const uint32_t taddr = tmem_base + lane_base + buf * kBN;
+            const float sx = row < a.rows ? a.x_scale[row] : 0.0f;
+#pragma unroll 1
+            for (int c = 0; c < kCols / 32; ++c) {
+                uint32_t acc[32], acc2[32];
+                tmem_ld32(taddr + c * 32, acc);
+                if (kGated) tmem_ld32(taddr + kBN / 2 + c * 32, acc2);
+                tmem_wait_ld();
+                const int col = n0 + c * 32;
+                if (row >= a.rows) continue;
+                const size_t o = (size_t)row * n_cols + col;
+                auto value = [&](int i, float sw, float sw2) {
+                    const float v = (float)(int)acc[i] * sx * sw;
+                    return kGated ? gated(v, (float)(int)acc2[i] * sx * sw2) : v;
+                };
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {              // eight columns at a time
+                    if (wide && col + 8 * p < n_cols) {
+                        float sw[8], sw2[8];
+                        *reinterpret_cast<float4*>(sw) = __ldg(reinterpret_cast<const float4*>(a.w_scale[0] + col + 8 * p));
+                        *reinterpret_cast<float4*>(sw + 4) = __ldg(reinterpret_cast<const float4*>(a.w_scale[0] + col + 8 * p) + 1);
+                        if (kGated) {
+                            *reinterpret_cast<float4*>(sw2) = __ldg(reinterpret_cast<const float4*>(a.w_scale[1] + col + 8 * p));
+                            *reinterpret_cast<float4*>(sw2 + 4) = __ldg(reinterpret_cast<const float4*>(a.w_scale[1] + col + 8 * p) + 1);
+                        }
+                        uint4 bias4 = make_uint4(0u, 0u, 0u, 0u), res4 = make_uint4(0u, 0u, 0u, 0u);
+                        if (a.bias[0]) bias4 = __ldg(reinterpret_cast<const uint4*>(a.bias[0] + col) + p);
+                        if (a.residual) res4 = *(reinterpret_cast<const uint4*>(a.residual + o) + p);
+                        const uint32_t* bw = reinterpret_cast<const uint32_t*>(&bias4);
+                        const uint32_t* rw = reinterpret_cast<const uint32_t*>(&res4);
+                        uint32_t packed[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float lo = value(8 * p + 2 * i, sw[2 * i], kGated ? sw2[2 * i] : 0.0f);
+                            float hi = value(8 * p + 2 * i + 1, sw[2 * i + 1], kGated ? sw2[2 * i + 1] : 0.0f);
+                            if (!kGated) {
+                                lo += bf16_lo(bw[i]) + bf16_lo(rw[i]);
+                                hi += bf16_hi(bw[i]) + bf16_hi(rw[i]);
+                            }
+                            packed[i] = pack_bf16x2(lo, hi);
+                        }
+                        *(reinterpret_cast<uint4*>(a.out[0] + o) + p) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+                    } else if (!wide) {
+#pragma unroll
+                        for (int i = 8 * p; i < 8 * p + 8; ++i) {
+                            if (col + i >= n_cols) continue;
+                            float v = value(i, __ldg(a.w_scale[0] + col + i), kGated ? __ldg(a.w_scale[1] + col + i) : 0.0f);
+                            if (a.bias[0]) v += bf16_bits_to_f32(__ldg(a.bias[0] + col + i));
+                            if (a.residual) v += bf16_bits_to_f32(a.residual[o + i]);
+                            a.out[0][o + i] = (uint16_t)f32_to_bf16_bits(v);
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+            mbar_arrive(acc_empty(buf));
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 4) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 2 * kBN);
+    }
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------
+
+// [rows][cols] 8-bit row-major viewed as {cols, rows}; boxes of box_rows x 128 columns, 128-byte swizzle, zeros outside.
+int32_t encode_byte_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return qm_fail(QM_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[2] = {cols, rows};
+    const cuuint64_t strides[1] = {cols};
+    const cuuint32_t box[2] = {kChunk, box_rows};
+    const cuuint32_t elem[2] = {1, 1};
+    const CUresult rc = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return qm_fail(QM_ECUDA, "cuTensorMapEncodeTiled failed for an 8-bit projection operand");
+    return QM_OK;
+}
+
+struct Int8Segment {
+    const int8_t* weight;
+    const float* scale;
+    const uint16_t* bias;
+    uint16_t* out;
+    int out_cols;
+};
+
+// CTAs that share a tile's K range: enough of them for two per SM, a power of two up to 8, two chunks each at least.
+int int8_split(int tiles, int chunks, int sms) {
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= 2 * sms && chunks / (split * 2) >= 2) split *= 2;
+    return split;
+}
+
+template <int kMPad, bool kGated>
+int32_t launch_skinny(const CUtensorMap* maps, const CUtensorMap& x_map, const Int8Args& a, unsigned grid, cudaStream_t stream,
+                      const char* what) {
+    auto kernel = qm_skinny_int8_kernel<kMPad, kGated>;
+    const size_t smem = SkinnySmem<kMPad>::kTotal + 1024;
+    QM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), what);
+    QM_CUDA_TRY(launch_cluster(kernel, dim3(grid), dim3(kProductThreads), (unsigned)a.split, smem, stream, maps[0], maps[1],
+                               maps[2], x_map, a),
+                what);
+    return QM_OK;
+}
+
+template <int kBN, bool kGated>
+int32_t launch_rows(const int8_t* x, const int8_t* w0, const int8_t* w1, Int8Args& a, int sms, cudaStream_t stream, const char* what) {
+    constexpr int kCols = kGated ? kBN / 2 : kBN;
+    CUtensorMap x_map, w0_map, w1_map;
+    int32_t rc = encode_byte_map(&x_map, x, (uint64_t)a.rows, (uint64_t)a.k_dim, 128);
+    if (rc == QM_OK) rc = encode_byte_map(&w0_map, w0, (uint64_t)a.out_cols[0], (uint64_t)a.k_dim, kBN / 2);
+    if (rc == QM_OK) rc = encode_byte_map(&w1_map, w1, (uint64_t)a.out_cols[0], (uint64_t)a.k_dim, kBN / 2);
+    if (rc != QM_OK) return rc;
+    a.n_tiles = (a.out_cols[0] + kCols - 1) / kCols;
+    const long long tiles = (long long)a.m_tiles * a.n_tiles;
+    if (tiles > 0x7fffffffLL) return qm_fail(QM_ECAPACITY, "too many output tiles for one launch");
+    auto kernel = qm_rows_int8_kernel<kBN, kGated>;
+    const size_t smem = RowsSmem<kBN>::kTotal + 1024;
+    QM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), what);
+    QM_CUDA_TRY(qm_launch(kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kProductThreads), smem, stream, x_map, w0_map,
+                          w1_map, a),
+                what);
+    return QM_OK;
+}
+
+template <bool kGated>
+int32_t run_int8(qm_kv_pool* pool, const int8_t* x, const float* x_scale, const Int8Segment* segs, int n_segs, const int8_t* up,
+                 const float* up_scale, const uint16_t* residual, int rows, int k_dim, cudaStream_t stream, const char* what) {
+    if (!pool) return qm_fail(QM_EINVAL, "pool is null");
+    if (rows < 0) return qm_fail(QM_EINVAL, "rows must be >= 0");
+    if (k_dim < 16 || k_dim % 16 != 0 || k_dim > 65536)
+        return qm_fail(QM_EINVAL, "reduction width must be a positive multiple of 16, at most 65536");
+    for (int i = 0; i < n_segs; ++i)
+        if (segs[i].out_cols < 1) return qm_fail(QM_EINVAL, "output width must be positive");
+    if (rows == 0) return QM_OK;                      // nothing to do; the row tensors may then be null
+    if (!x || !x_scale || (kGated && (!up || !up_scale))) return qm_fail(QM_EINVAL, "null tensor pointer");
+    uintptr_t all = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(up) | reinterpret_cast<uintptr_t>(up_scale) |
+                    reinterpret_cast<uintptr_t>(residual);
+    for (int i = 0; i < n_segs; ++i) {
+        if (!segs[i].weight || !segs[i].scale || !segs[i].out) return qm_fail(QM_EINVAL, "null tensor pointer");
+        all |= reinterpret_cast<uintptr_t>(segs[i].weight) | reinterpret_cast<uintptr_t>(segs[i].scale) |
+               reinterpret_cast<uintptr_t>(segs[i].bias) | reinterpret_cast<uintptr_t>(segs[i].out);
+    }
+    if ((all & 15u) || (reinterpret_cast<uintptr_t>(x_scale) & 3u))
+        return qm_fail(QM_EINVAL, "8-bit projection operands must be 16-byte aligned");
+    int device = -1;
+    QM_CUDA_TRY(cudaGetDevice(&device), "get current device");
+    if (device != pool->device) return qm_fail(QM_EINVAL, "the pool's device must be the current device");
+
+    Int8Args a{};
+    a.x_scale = x_scale;
+    a.residual = residual;
+    a.status = pool->status_dev;
+    a.rows = rows;
+    a.k_dim = k_dim;
+    a.chunks = (k_dim + kChunk - 1) / kChunk;
+    const int sms = pool->sm_count;
+    if (rows <= 64) {
+        const int rows_per_tile = kGated ? 64 : kWeightRows;
+        CUtensorMap maps[3], x_map;
+        int tiles = 0;
+        for (int i = 0; i < 3; ++i) {
+            const Int8Segment& sg = segs[i < n_segs ? i : n_segs - 1];
+            const bool second = kGated && i == 1;
+            a.weight[i] = second ? up : sg.weight;
+            a.w_scale[i] = second ? up_scale : sg.scale;
+            a.first_tile[i] = i < n_segs ? tiles : 0x7fffffff;
+            const int32_t rc = encode_byte_map(&maps[i], a.weight[i], (uint64_t)sg.out_cols, (uint64_t)k_dim, (uint32_t)rows_per_tile);
+            if (rc != QM_OK) return rc;
+            if (i < n_segs) {
+                a.bias[i] = sg.bias;
+                a.out[i] = sg.out;
+                a.out_cols[i] = sg.out_cols;
+                tiles += (sg.out_cols + rows_per_tile - 1) / rows_per_tile;
+            }
+        }
+        const int m_pad = rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
+        const int32_t rc = encode_byte_map(&x_map, x, (uint64_t)rows, (uint64_t)k_dim, (uint32_t)m_pad);
+        if (rc != QM_OK) return rc;
+        a.split = int8_split(tiles, a.chunks, sms);
+        const unsigned grid = (unsigned)tiles * (unsigned)a.split;
+        if (m_pad == 16) return launch_skinny<16, kGated>(maps, x_map, a, grid, stream, what);
+        if (m_pad == 32) return launch_skinny<32, kGated>(maps, x_map, a, grid, stream, what);
+        return launch_skinny<64, kGated>(maps, x_map, a, grid, stream, what);
+    }
+    a.m_tiles = (rows + 127) / 128;
+    for (int i = 0; i < n_segs; ++i) {
+        a.weight[0] = segs[i].weight;
+        a.w_scale[0] = segs[i].scale;
+        a.w_scale[1] = up_scale;
+        a.bias[0] = segs[i].bias;
+        a.out[0] = segs[i].out;
+        a.out_cols[0] = segs[i].out_cols;
+        // the widest tile that still gives every SM one
+        auto enough = [&](int bn) {
+            const int cols = kGated ? bn / 2 : bn;
+            return (long long)a.m_tiles * ((segs[i].out_cols + cols - 1) / cols) >= sms;
+        };
+        const int8_t* second = kGated ? up : segs[i].weight;
+        int32_t rc;
+        if (enough(256)) rc = launch_rows<256, kGated>(x, segs[i].weight, second, a, sms, stream, what);
+        else if (enough(128)) rc = launch_rows<128, kGated>(x, segs[i].weight, second, a, sms, stream, what);
+        else rc = launch_rows<64, kGated>(x, segs[i].weight, second, a, sms, stream, what);
+        if (rc != QM_OK) return rc;
+    }
+    return QM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t qm_quantize_rows_int8(const uint16_t* x, const uint16_t* norm_weight, float epsilon, int8_t* q, float* scale, int32_t rows,
+                              int32_t dim, void* stream) {
+    if (rows < 0 || dim < 1 || dim > kQuantMaxDim) return qm_fail(QM_EINVAL, "dim must be between 1 and 24576");
+    if (rows == 0) return QM_OK;
+    if (!x || !q || !scale) return qm_fail(QM_EINVAL, "null tensor pointer");
+    const uintptr_t bf16s = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(norm_weight);
+    if ((bf16s & 1u) || (reinterpret_cast<uintptr_t>(scale) & 3u)) return qm_fail(QM_EINVAL, "misaligned tensor pointer");
+    const size_t smem = ((size_t)dim * 2 + 15) / 16 * 16;
+    const bool vector = dim % 8 == 0 && (bf16s & 15u) == 0 && (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
+    auto kernel = vector ? qm_quantize_rows_kernel<true> : qm_quantize_rows_kernel<false>;
+    if (smem > 47 * 1024)         // the row and the static words together pass the 48 KB that need no opt-in
+        QM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kQuantMaxDim * 2),
+                    "raise row quantisation shared memory");
+    QM_CUDA_TRY(qm_launch(kernel, dim3((unsigned)rows), dim3(kQuantThreads), smem, static_cast<cudaStream_t>(stream), x, norm_weight,
+                          epsilon, q, scale, (int)dim),
+                "row quantisation launch");
+    return QM_OK;
+}
+
+int32_t qm_linear_int8(qm_kv_pool* pool, const int8_t* x, const float* x_scale, const int8_t* weight, const float* weight_scale,
+                       const uint16_t* bias, const uint16_t* residual, uint16_t* out, int32_t rows, int32_t out_features,
+                       int32_t in_features, void* stream) {
+    const Int8Segment seg{weight, weight_scale, bias, out, out_features};
+    return run_int8<false>(pool, x, x_scale, &seg, 1, nullptr, nullptr, residual, rows, in_features,
+                           static_cast<cudaStream_t>(stream), "8-bit projection launch");
+}
+
+int32_t qm_qkv_linear_int8(qm_kv_pool* pool, const int8_t* x, const float* x_scale, const int8_t* q_weight, const float* q_scale,
+                           const uint16_t* q_bias, const int8_t* k_weight, const float* k_scale, const uint16_t* k_bias,
+                           const int8_t* v_weight, const float* v_scale, const uint16_t* v_bias, uint16_t* q_out, uint16_t* k_out,
+                           uint16_t* v_out, int32_t rows, int32_t hidden, int32_t q_dim, int32_t kv_dim, void* stream) {
+    const Int8Segment segs[3] = {{q_weight, q_scale, q_bias, q_out, q_dim},
+                                 {k_weight, k_scale, k_bias, k_out, kv_dim},
+                                 {v_weight, v_scale, v_bias, v_out, kv_dim}};
+    return run_int8<false>(pool, x, x_scale, segs, 3, nullptr, nullptr, nullptr, rows, hidden, static_cast<cudaStream_t>(stream),
+                           "8-bit QKV projection launch");
+}
+
+int32_t qm_gate_up_swiglu_int8(qm_kv_pool* pool, const int8_t* x, const float* x_scale, const int8_t* gate_weight,
+                               const float* gate_scale, const int8_t* up_weight, const float* up_scale, uint16_t* out, int32_t rows,
+                               int32_t hidden, int32_t intermediate, void* stream) {
+    const Int8Segment seg{gate_weight, gate_scale, nullptr, out, intermediate};
+    return run_int8<true>(pool, x, x_scale, &seg, 1, up_weight, up_scale, nullptr, rows, hidden, static_cast<cudaStream_t>(stream),
+                          "8-bit gate/up/SwiGLU launch");
+}
+
+}  // extern "C"

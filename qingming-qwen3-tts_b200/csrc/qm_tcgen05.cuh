@@ -38,6 +38,15 @@ __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_
         : "memory");
 }
 
+// D[tmem] (+)= A[smem] * B[smem] on 8-bit integers, exact 32-bit sums (K = 32 per instruction)
+__device__ __forceinline__ void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -112,6 +121,15 @@ __host__ __device__ constexpr uint32_t umma_instr_desc(int m, int n, bool b_mn_m
            | (1u << 7)                    // A format BF16
            | (1u << 10)                   // B format BF16
            | ((b_mn_major ? 1u : 0u) << 16)
+           | ((uint32_t)(n >> 3) << 17)
+           | ((uint32_t)(m >> 4) << 24);
+}
+
+// Instruction descriptor: signed 8-bit x signed 8-bit -> 32-bit integer sums, both operands K-major.
+__host__ __device__ constexpr uint32_t umma_instr_desc_s8(int m, int n) {
+    return (2u << 4)                      // accumulator format S32
+           | (1u << 7)                    // A format signed 8-bit
+           | (1u << 10)                   // B format signed 8-bit
            | ((uint32_t)(n >> 3) << 17)
            | ((uint32_t)(m >> 4) << 24);
 }

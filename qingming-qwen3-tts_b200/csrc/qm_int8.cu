@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kQuantThreads) qm_quantize_rows_kernel(const u
 // ---- shared by the two products -----------------------------------------------------------------------------------
 
 constexpr int kChunk = 128;                    // K columns (bytes) per ring stage: one 128-byte swizzle atom
-constexpr int kProductThreads = 192;           // warps 0-3 epilogue, warp 4 MMA issue, warp 5 TMA
+constexpr int kSkinnyThreads = 192;            // warps 0-3 epilogue, warp 4 MMA issue, warp 5 TMA
 constexpr int kWeightRows = 128;
 
 // gate * sigmoid(gate) * up in fp32
@@ -203,7 +203,7 @@ __device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t remote_addr) {
 }
 
 template <int kMPad, bool kGated>
-__global__ void __launch_bounds__(kProductThreads)
+__global__ void __launch_bounds__(kSkinnyThreads)
 qm_skinny_int8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap w2_map,
                       const __grid_constant__ CUtensorMap w3_map, const __grid_constant__ CUtensorMap x_map, const Int8Args a) {
     using L = SkinnySmem<kMPad>;
@@ -382,22 +382,37 @@ qm_skinny_int8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_co
 // ---- more token rows ------------------------------------------------------------------------------------------------
 //
 // One CTA per SM walks tiles of 128 token rows x kBN weight rows (gated: kBN / 2 gate rows and the same up rows); the
-// MMA thread fills one TMEM accumulator while the epilogue warps drain the other.  kBN = 256 has the fewest
-// operand bytes per operation; the narrower tiles are for calls whose 256-wide tiles would leave SMs without one.
+// MMA thread fills one TMEM accumulator while eight epilogue warps drain the other (two warps per quarter of the
+// lanes, alternate blocks of 32 columns).  The tile's column scales and biases are fetched into shared memory while
+// its products are still running; results leave through a 2 KB block per warp and TMA stores, which also clip the
+// last tile.  kBN = 256 has the fewest operand bytes per operation; the narrower tiles are for calls whose 256-wide
+// tiles would leave SMs without one.
+constexpr int kRowsThreads = 320;              // warps 0-7 epilogue, warp 8 MMA issue, warp 9 TMA loads
+constexpr int kRowsEpilogue = 256;
+constexpr int kStoreBytes = 32 * 32 * 2;       // 32 rows x 32 bf16 columns, 64-byte swizzle
+
 template <int kBN>
 struct RowsSmem {
     static constexpr int kStageA = 128 * kChunk;
     static constexpr int kStageBytes = kStageA + kBN * kChunk;
     static constexpr int kStages = kBN == 256 ? 4 : (kBN == 128 ? 6 : 8);
-    static constexpr int kBars = kStages * kStageBytes;                    // full, empty, acc_full[2], acc_empty[2]
+    static constexpr int kStore = kStages * kStageBytes;                   // one block per epilogue warp
+    static constexpr int kColumns = kStore + 8 * kStoreBytes;              // float[2][3][kBN]: scale, up scale, bias
+    static constexpr int kBars = kColumns + 2 * 3 * kBN * 4;               // full, empty, acc_full[2], acc_empty[2]
     static constexpr int kTmemSlot = kBars + (2 * kStages + 4) * 8;
     static constexpr int kTotal = kTmemSlot + 16;
+    static_assert(kTotal + 1024 <= 227 * 1024, "shared memory of one CTA");
 };
 
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(x), "r"(y)
+                 : "memory");
+}
+
 template <int kBN, bool kGated>
-__global__ void __launch_bounds__(kProductThreads, 1)
+__global__ void __launch_bounds__(kRowsThreads, 1)
 qm_rows_int8_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w0_map,
-                    const __grid_constant__ CUtensorMap w1_map, const Int8Args a) {
+                    const __grid_constant__ CUtensorMap w1_map, const __grid_constant__ CUtensorMap out_map, const Int8Args a) {
     using L = RowsSmem<kBN>;
     constexpr int kCols = kGated ? kBN / 2 : kBN;           // output columns per tile
     pdl_trigger();
@@ -421,11 +436,11 @@ qm_rows_int8_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full(b), 1);
-            mbar_init(acc_empty(b), 128);
+            mbar_init(acc_empty(b), kRowsEpilogue);
         }
         fence_mbar_init();
     }
-    if (warp == 4) {
+    if (warp == 8) {
         tmem_alloc(smem_addr(tmem_slot), 2 * kBN);
         tmem_relinquish();
     }
@@ -437,7 +452,7 @@ qm_rows_int8_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
     bool dead = false;
     pdl_wait();
 
-    if (warp == 5) {
+    if (warp == 9) {
         if (lane == 0) {
             int it = 0;
             for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x) {
@@ -459,7 +474,7 @@ qm_rows_int8_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
             drain_ring(full_bar, it, L::kStages);
         }
         __syncwarp();
-    } else if (warp == 4) {
+    } else if (warp == 8) {
         if (lane == 0) {
             constexpr uint32_t idesc = umma_instr_desc_s8(128, kBN);
             int it = 0, local = 0;
@@ -486,79 +501,100 @@ qm_rows_int8_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
         }
         __syncwarp();
     } else {
-        const int row_in_tile = warp * 32 + lane;
-        const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+        const int quarter = warp & 3;                      // which TMEM lanes this warp may read
+        const int row_in_tile = quarter * 32 + lane;
+        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         const int n_cols = a.out_cols[0];
-        const bool wide = (n_cols & 7) == 0;               // every 8-column piece of a row is then 16-byte aligned
+        const bool wide = (n_cols & 7) == 0;               // rows are 16-byte multiples: TMA stores, 16-byte loads
+        const uint32_t block = sbase + L::kStore + warp * kStoreBytes;
+        const uint32_t my_row = block + lane * 64;
+        const uint32_t swizzle = (uint32_t)((lane >> 1) & 3);       // 64-byte swizzle: 16-byte piece ^ (row / 2) % 4
+        float* columns = reinterpret_cast<float*>(smem + L::kColumns);
         int local = 0;
         for (int tile = blockIdx.x; tile < total_tiles; tile += gridDim.x, ++local) {
             const int buf = local & 1;
             const int n0 = (tile % a.n_tiles) * kCols;
-            const int row = (tile / a.n_tiles) * 128 + row_in_tile;
+            const int m0 = (tile / a.n_tiles) * 128;
+            const int row = m0 + row_in_tile;
+            float* cs = columns + buf * 3 * kBN;           // two buffers: the other one may still be read
+            if (tid < kCols) {
+                const bool in = n0 + tid < n_cols;
+                cs[tid] = in ? __ldg(a.w_scale[0] + n0 + tid) : 0.0f;
+                if (kGated) cs[kBN + tid] = in ? __ldg(a.w_scale[1] + n0 + tid) : 0.0f;
+                if (!kGated) cs[2 * kBN + tid] = in && a.bias[0] ? bf16_bits_to_f32(__ldg(a.bias[0] + n0 + tid)) : 0.0f;
+            }
+            const float sx = row < a.rows ? a.x_scale[row] : 0.0f;
+            named_bar_sync(1, kRowsEpilogue);
             if (!mbar_wait_bounded(acc_full(buf), (local >> 1) & 1, dead) && lane == 0) atomicOr(a.status, QM_DEVSTAT_TIMEOUT);
             tc_fence_after();
             const uint32_t taddr = tmem_base + lane_base + buf * kBN;
-            const float sx = row < a.rows ? a.x_scale[row] : 0.0f;
 #pragma unroll 1
-            for (int c = 0; c < kCols / 32; ++c) {
+            for (int c = warp >> 2; c < kCols / 32; c += 2) {
+                const int col = n0 + c * 32;
+                if (col >= n_cols) break;
                 uint32_t acc[32], acc2[32];
                 tmem_ld32(taddr + c * 32, acc);
                 if (kGated) tmem_ld32(taddr + kBN / 2 + c * 32, acc2);
-                tmem_wait_ld();
-                const int col = n0 + c * 32;
-                if (row >= a.rows) continue;
                 const size_t o = (size_t)row * n_cols + col;
-                auto value = [&](int i, float sw, float sw2) {
-                    const float v = (float)(int)acc[i] * sx * sw;
-                    return kGated ? gated(v, (float)(int)acc2[i] * sx * sw2) : v;
-                };
+                uint4 res[4];
+                const bool vector_residual = !kGated && wide && a.residual != nullptr;
 #pragma unroll
-                for (int p = 0; p < 4; ++p) {              // eight columns at a time
-                    if (wide && col + 8 * p < n_cols) {
-                        float sw[8], sw2[8];
-                        *reinterpret_cast<float4*>(sw) = __ldg(reinterpret_cast<const float4*>(a.w_scale[0] + col + 8 * p));
-                        *reinterpret_cast<float4*>(sw + 4) = __ldg(reinterpret_cast<const float4*>(a.w_scale[0] + col + 8 * p) + 1);
-                        if (kGated) {
-                            *reinterpret_cast<float4*>(sw2) = __ldg(reinterpret_cast<const float4*>(a.w_scale[1] + col + 8 * p));
-                            *reinterpret_cast<float4*>(sw2 + 4) = __ldg(reinterpret_cast<const float4*>(a.w_scale[1] + col + 8 * p) + 1);
-                        }
-                        uint4 bias4 = make_uint4(0u, 0u, 0u, 0u), res4 = make_uint4(0u, 0u, 0u, 0u);
-                        if (a.bias[0]) bias4 = __ldg(reinterpret_cast<const uint4*>(a.bias[0] + col) + p);
-                        if (a.residual) res4 = *(reinterpret_cast<const uint4*>(a.residual + o) + p);
-                        const uint32_t* bw = reinterpret_cast<const uint32_t*>(&bias4);
-                        const uint32_t* rw = reinterpret_cast<const uint32_t*>(&res4);
-                        uint32_t packed[4];
+                for (int p = 0; p < 4; ++p)
+                    res[p] = vector_residual && row < a.rows && col + 8 * p < n_cols ? *(reinterpret_cast<const uint4*>(a.residual + o) + p)
+                                                                                     : make_uint4(0u, 0u, 0u, 0u);
+                tmem_wait_ld();
+                uint32_t packed[16];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float lo = value(8 * p + 2 * i, sw[2 * i], kGated ? sw2[2 * i] : 0.0f);
-                            float hi = value(8 * p + 2 * i + 1, sw[2 * i + 1], kGated ? sw2[2 * i + 1] : 0.0f);
-                            if (!kGated) {
-                                lo += bf16_lo(bw[i]) + bf16_lo(rw[i]);
-                                hi += bf16_hi(bw[i]) + bf16_hi(rw[i]);
-                            }
-                            packed[i] = pack_bf16x2(lo, hi);
-                        }
-                        *(reinterpret_cast<uint4*>(a.out[0] + o) + p) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-                    } else if (!wide) {
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 sw = *reinterpret_cast<const float2*>(cs + c * 32 + i);
+                    float2 v = make_float2((float)(int)acc[i] * sx * sw.x, (float)(int)acc[i + 1] * sx * sw.y);
+                    if (kGated) {
+                        const float2 su = *reinterpret_cast<const float2*>(cs + kBN + c * 32 + i);
+                        v.x = gated(v.x, (float)(int)acc2[i] * sx * su.x);
+                        v.y = gated(v.y, (float)(int)acc2[i + 1] * sx * su.y);
+                    } else {
+                        const float2 bias = *reinterpret_cast<const float2*>(cs + 2 * kBN + c * 32 + i);
+                        const uint32_t rw = reinterpret_cast<const uint32_t*>(res)[i >> 1];
+                        v = make_float2(v.x + bias.x + bf16_lo(rw), v.y + bias.y + bf16_hi(rw));
+                    }
+                    if (wide) {
+                        packed[i >> 1] = pack_bf16x2(v.x, v.y);
+                    } else if (row < a.rows) {
 #pragma unroll
-                        for (int i = 8 * p; i < 8 * p + 8; ++i) {
-                            if (col + i >= n_cols) continue;
-                            float v = value(i, __ldg(a.w_scale[0] + col + i), kGated ? __ldg(a.w_scale[1] + col + i) : 0.0f);
-                            if (a.bias[0]) v += bf16_bits_to_f32(__ldg(a.bias[0] + col + i));
-                            if (a.residual) v += bf16_bits_to_f32(a.residual[o + i]);
-                            a.out[0][o + i] = (uint16_t)f32_to_bf16_bits(v);
+                        for (int h = 0; h < 2; ++h) {
+                            if (col + i + h >= n_cols) continue;
+                            float one = h ? v.y : v.x;
+                            if (!kGated && a.residual) one += bf16_bits_to_f32(a.residual[o + i + h]);
+                            a.out[0][o + i + h] = (uint16_t)f32_to_bf16_bits(one);
                         }
+                    }
+                }
+                if (wide) {
+                    // the warp's previous block has been read by its store
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    __syncwarp();
+#pragma unroll
+                    for (int p = 0; p < 4; ++p)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(my_row + (((uint32_t)p ^ swizzle) << 4)),
+                                     "r"(packed[4 * p]), "r"(packed[4 * p + 1]), "r"(packed[4 * p + 2]), "r"(packed[4 * p + 3])
+                                     : "memory");
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0 && m0 + quarter * 32 < a.rows) {
+                        tma_store_2d(&out_map, block, col, m0 + quarter * 32);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
                 }
             }
             tc_fence_before();
             mbar_arrive(acc_empty(buf));
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 
     tc_fence_before();
     __syncthreads();
-    if (warp == 4) {
+    if (warp == 8) {
         tc_fence_after();
         tmem_dealloc(tmem_base, 2 * kBN);
     }
@@ -578,6 +614,20 @@ int32_t encode_byte_map(CUtensorMap* map, const void* base, uint64_t rows, uint6
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) return qm_fail(QM_ECUDA, "cuTensorMapEncodeTiled failed for an 8-bit projection operand");
+    return QM_OK;
+}
+
+// [rows][cols] bf16 results: blocks of 32 x 32, 64-byte swizzle.
+int32_t encode_result_map(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return qm_fail(QM_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[2] = {cols, rows};
+    const cuuint64_t strides[1] = {cols * 2};
+    const cuuint32_t box[2] = {32, 32};
+    const cuuint32_t elem[2] = {1, 1};
+    const CUresult rc = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return qm_fail(QM_ECUDA, "cuTensorMapEncodeTiled failed for a projection result");
     return QM_OK;
 }
 
@@ -602,7 +652,7 @@ int32_t launch_skinny(const CUtensorMap* maps, const CUtensorMap& x_map, const I
     auto kernel = qm_skinny_int8_kernel<kMPad, kGated>;
     const size_t smem = SkinnySmem<kMPad>::kTotal + 1024;
     QM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), what);
-    QM_CUDA_TRY(launch_cluster(kernel, dim3(grid), dim3(kProductThreads), (unsigned)a.split, smem, stream, maps[0], maps[1],
+    QM_CUDA_TRY(launch_cluster(kernel, dim3(grid), dim3(kSkinnyThreads), (unsigned)a.split, smem, stream, maps[0], maps[1],
                                maps[2], x_map, a),
                 what);
     return QM_OK;
@@ -611,10 +661,11 @@ int32_t launch_skinny(const CUtensorMap* maps, const CUtensorMap& x_map, const I
 template <int kBN, bool kGated>
 int32_t launch_rows(const int8_t* x, const int8_t* w0, const int8_t* w1, Int8Args& a, int sms, cudaStream_t stream, const char* what) {
     constexpr int kCols = kGated ? kBN / 2 : kBN;
-    CUtensorMap x_map, w0_map, w1_map;
+    CUtensorMap x_map, w0_map, w1_map, out_map{};
     int32_t rc = encode_byte_map(&x_map, x, (uint64_t)a.rows, (uint64_t)a.k_dim, 128);
     if (rc == QM_OK) rc = encode_byte_map(&w0_map, w0, (uint64_t)a.out_cols[0], (uint64_t)a.k_dim, kBN / 2);
     if (rc == QM_OK) rc = encode_byte_map(&w1_map, w1, (uint64_t)a.out_cols[0], (uint64_t)a.k_dim, kBN / 2);
+    if (rc == QM_OK && a.out_cols[0] % 8 == 0) rc = encode_result_map(&out_map, a.out[0], (uint64_t)a.rows, (uint64_t)a.out_cols[0]);
     if (rc != QM_OK) return rc;
     a.n_tiles = (a.out_cols[0] + kCols - 1) / kCols;
     const long long tiles = (long long)a.m_tiles * a.n_tiles;
@@ -622,8 +673,8 @@ int32_t launch_rows(const int8_t* x, const int8_t* w0, const int8_t* w1, Int8Arg
     auto kernel = qm_rows_int8_kernel<kBN, kGated>;
     const size_t smem = RowsSmem<kBN>::kTotal + 1024;
     QM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), what);
-    QM_CUDA_TRY(qm_launch(kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kProductThreads), smem, stream, x_map, w0_map,
-                          w1_map, a),
+    QM_CUDA_TRY(qm_launch(kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kRowsThreads), smem, stream, x_map, w0_map,
+                          w1_map, out_map, a),
                 what);
     return QM_OK;
 }

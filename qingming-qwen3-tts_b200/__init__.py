@@ -176,7 +176,8 @@ def _shaped(what: str, tensor, *shape) -> None:
 def _stream() -> int:
     import torch
 
-    return torch.cuda.current_stream().cuda_stream
+    # current_stream() builds a Stream object around this number, which takes as long as a kernel launch
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 class TalkerAttention:
@@ -388,8 +389,8 @@ class TalkerAttention:
         import torch
 
         rows, dim = x.shape
-        q = torch.empty((rows, dim), dtype=torch.int8, device=x.device) if q is None else q
-        scale = torch.empty((rows,), dtype=torch.float32, device=x.device) if scale is None else scale
+        q = x.new_empty((rows, dim), dtype=torch.int8) if q is None else q
+        scale = x.new_empty((rows,), dtype=torch.float32) if scale is None else scale
         _packed(torch.bfloat16, x, norm_weight)
         _packed(torch.int8, q)
         _packed(torch.float32, scale)
@@ -405,7 +406,7 @@ class TalkerAttention:
 
         rows, inner = x.shape
         outer = weight.shape[0]
-        out = torch.empty((rows, outer), dtype=torch.bfloat16, device=x.device) if out is None else out
+        out = x.new_empty((rows, outer), dtype=torch.bfloat16) if out is None else out
         _packed(torch.int8, x, weight)
         _packed(torch.float32, x_scale, weight_scale)
         _packed(torch.bfloat16, bias, residual, out)
@@ -426,7 +427,7 @@ class TalkerAttention:
 
         rows, inner = x.shape
         if out is None:
-            out = tuple(torch.empty((rows, w.shape[0]), dtype=torch.bfloat16, device=x.device) for w in (q_weight, k_weight, v_weight))
+            out = tuple(x.new_empty((rows, w.shape[0]), dtype=torch.bfloat16) for w in (q_weight, k_weight, v_weight))
         _packed(torch.int8, x, q_weight, k_weight, v_weight)
         _packed(torch.float32, x_scale, q_scale, k_scale, v_scale)
         _packed(torch.bfloat16, q_bias, k_bias, v_bias, *out)
@@ -450,7 +451,7 @@ class TalkerAttention:
 
         rows, inner = x.shape
         outer = gate_weight.shape[0]
-        out = torch.empty((rows, outer), dtype=torch.bfloat16, device=x.device) if out is None else out
+        out = x.new_empty((rows, outer), dtype=torch.bfloat16) if out is None else out
         _packed(torch.int8, x, gate_weight, up_weight)
         _packed(torch.float32, x_scale, gate_scale, up_scale)
         _packed(torch.bfloat16, out)

@@ -22,126 +22,189 @@ namespace {
 
 // ---- quantisation of rows -----------------------------------------------------------------------------------------
 
-constexpr int kQuantThreads = 256;
+constexpr int kQuantThreads = 256;             // CTA per row
+constexpr int kQuantWarps = 8;                 // warp per row
 constexpr int kQuantMaxDim = 24 * 1024;        // the row is staged in shared memory as bf16
 
-// One row.  With a norm weight the value quantised is n[k] = x[k] * w[k] / rms; the rms divides out of q (q is a ratio
-// of two such values) and enters the scale alone, so one sweep collects both the sum of squares and the largest
-// |x w|, and x w is exact in fp32 (two 8-bit significands).  A power of two keeps very large and very small rows
-// inside fp32's range.  A row with an infinity or a NaN gets scale NaN and q = 0: every output of that row is NaN.
-struct QuantRow {
-    float pre;          // exact power of two applied to the values
-    float ratio;        // 127 / (largest * pre)
-    float largest;      // largest * pre
+// With a norm weight the value quantised is v[k] = x[k] * w[k] / rms; the rms divides out of q (q is a ratio of two such
+// values) and enters the scale alone, so one sweep collects both the sum of squares and the largest |x w|, and x w is
+// exact in fp32 (two 8-bit significands).  The largest magnitude is taken over the bit patterns, where an infinity or a
+// NaN is larger than any number.
+struct RowSweep {
+    float sum;
+    uint32_t big_bits;
 };
 
-__device__ __forceinline__ int quantize_value(float v, const QuantRow& r) {
-    const float scaled = v * r.pre;
-    float t = scaled * r.ratio;
-    // The product is within 2e-5 of the quotient.  Only next to a half step can that change the rounding, and there
-    // the correctly rounded quotient decides (127 * scaled is exact: at most 7 + 16 bits).
-    if (fabsf(fabsf(t - rintf(t)) - 0.5f) < 1.0e-4f) t = __fdiv_rn(127.0f * scaled, r.largest);
-    return (int)rintf(t);
+struct QuantRow {
+    float ratio;        // 127 / big where that is an ordinary number
+    float big;
+    float pre;          // exact power of two that keeps 127 * v and big inside fp32's range
+    bool flat;          // nothing to quantise (all zero, or no scale): every q is zero
+    bool plain;         // pre is 1
+};
+
+template <bool kNorm>
+__device__ __forceinline__ void sweep_eight(const uint4& raw, const uint4& wv, RowSweep& s) {
+    const uint32_t* rw = reinterpret_cast<const uint32_t*>(&raw);
+    const uint32_t* ww = reinterpret_cast<const uint32_t*>(&wv);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float2 v = bf16x2_to_float2(rw[i]);
+        if (kNorm) {
+            s.sum = fmaf(v.x, v.x, fmaf(v.y, v.y, s.sum));
+            v = fmul2(v, bf16x2_to_float2(ww[i]));
+        }
+        s.big_bits = max(s.big_bits, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu));
+    }
 }
 
-template <bool kVector>
+__device__ __forceinline__ QuantRow quant_row(uint32_t big_bits) {
+    QuantRow r;
+    r.flat = big_bits == 0u || big_bits >= 0x7f800000u;
+    r.big = __uint_as_float(big_bits);
+    r.pre = r.big > 1.0e30f ? 0x1p-64f : (r.big < 1.0e-30f ? 0x1p64f : 1.0f);
+    r.plain = r.pre == 1.0f;
+    r.ratio = r.flat ? 0.0f : 127.0f / r.big;
+    return r;
+}
+
+__device__ __forceinline__ float row_scale(const QuantRow& r, float sum, bool norm, int dim, float epsilon) {
+    float s = r.big / 127.0f;
+    if (norm) s *= rsqrtf(sum / (float)dim + epsilon);
+    return r.flat && r.big != 0.0f ? CUDART_NAN_F : s;
+}
+
+// The correctly rounded quotient 127 v / big (the product is exact: at most 7 + 16 bits), to the nearest whole number.
+__device__ __forceinline__ int quantize_exactly(float v, const QuantRow& r) {
+    return (int)rintf(__fdiv_rn(127.0f * (v * r.pre), r.big * r.pre));
+}
+
+// Eight values at once.  fma(v, ratio, 1.5 * 2^23) leaves round(v * ratio) in the low bits; v * ratio is within 8e-6 of
+// the quotient (ratio's own rounding), which can only change the rounding right beside a half step: if any of the
+// eight is that near to one, all are divided.
+template <bool kNorm>
+__device__ __forceinline__ uint2 quantize_eight(const uint4& raw, const uint4& wv, const QuantRow& r) {
+    if (r.flat) return make_uint2(0u, 0u);
+    constexpr float kMagic = 12582912.0f;
+    const uint32_t* rw = reinterpret_cast<const uint32_t*>(&raw);
+    const uint32_t* ww = reinterpret_cast<const uint32_t*>(&wv);
+    float v[8];
+    uint32_t level[8];
+    float off = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float2 e = bf16x2_to_float2(rw[i]);
+        if (kNorm) e = fmul2(e, bf16x2_to_float2(ww[i]));
+        v[2 * i] = e.x;
+        v[2 * i + 1] = e.y;
+        const float2 ratio2 = make_float2(r.ratio, r.ratio);
+        const float2 m = ffma2(e, ratio2, make_float2(kMagic, kMagic));
+        const float2 back = fadd2(make_float2(kMagic, kMagic), make_float2(-m.x, -m.y));
+        const float2 d = ffma2(e, ratio2, back);
+        off = fmax3(off, fabsf(d.x), fabsf(d.y));
+        level[2 * i] = __float_as_uint(m.x);
+        level[2 * i + 1] = __float_as_uint(m.y);
+    }
+    if (off > 0.49995f || !r.plain) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) level[i] = (uint32_t)quantize_exactly(v[i], r);
+    }
+    uint2 packed;
+    packed.x = __byte_perm(__byte_perm(level[0], level[1], 0x0040), __byte_perm(level[2], level[3], 0x0040), 0x5410);
+    packed.y = __byte_perm(__byte_perm(level[4], level[5], 0x0040), __byte_perm(level[6], level[7], 0x0040), 0x5410);
+    return packed;
+}
+
+// A CTA per row: few rows, each as fast as it goes; any width and alignment (kVector = false).
+template <bool kVector, bool kNorm>
 __global__ void __launch_bounds__(kQuantThreads) qm_quantize_rows_kernel(const uint16_t* __restrict__ x,
                                                                         const uint16_t* __restrict__ norm_weight,
                                                                         float epsilon, int8_t* __restrict__ q,
                                                                         float* __restrict__ scale, int dim) {
     extern __shared__ uint4 row_vectors[];
-    __shared__ float warp_sum[kQuantThreads / 32], warp_max[kQuantThreads / 32];
-    __shared__ int warp_bad[kQuantThreads / 32];
+    __shared__ float warp_sum[kQuantThreads / 32];
+    __shared__ uint32_t warp_big[kQuantThreads / 32];
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const size_t base = (size_t)blockIdx.x * dim;
+    const uint4* weights = reinterpret_cast<const uint4*>(norm_weight);
     uint16_t* staged = reinterpret_cast<uint16_t*>(row_vectors);
-    float sum = 0.0f, big = 0.0f;
-    bool bad = false;
-    auto take = [&](float v, float w) {
-        sum = fmaf(v, v, sum);
-        const float m = fabsf(v * w);
-        bad |= !(m < CUDART_INF_F);
-        big = fmaxf(big, m);
-    };
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+    RowSweep s = {0.0f, 0u};
     if (kVector) {
         for (int v = tid; v < dim / 8; v += kQuantThreads) {
             const uint4 raw = *reinterpret_cast<const uint4*>(x + base + 8 * v);
             row_vectors[v] = raw;
-            uint4 wv = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);      // ones
-            if (norm_weight) wv = __ldg(reinterpret_cast<const uint4*>(norm_weight + 8 * v));
-            const uint32_t* rw = reinterpret_cast<const uint32_t*>(&raw);
-            const uint32_t* ww = reinterpret_cast<const uint32_t*>(&wv);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                take(bf16_lo(rw[i]), bf16_lo(ww[i]));
-                take(bf16_hi(rw[i]), bf16_hi(ww[i]));
-            }
+            sweep_eight<kNorm>(raw, kNorm ? __ldg(weights + v) : none, s);
         }
     } else {
         for (int c = tid; c < dim; c += kQuantThreads) {
             const uint16_t raw = x[base + c];
             staged[c] = raw;
-            take(bf16_bits_to_f32(raw), norm_weight ? bf16_bits_to_f32(norm_weight[c]) : 1.0f);
+            float v = bf16_bits_to_f32(raw);
+            s.sum = fmaf(v, v, s.sum);
+            if (kNorm) v *= bf16_bits_to_f32(norm_weight[c]);
+            s.big_bits = max(s.big_bits, __float_as_uint(v) & 0x7fffffffu);
         }
     }
+    s.big_bits = __reduce_max_sync(0xffffffffu, s.big_bits);
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-    }
-    bad = __any_sync(0xffffffffu, bad);
+    for (int off = 16; off > 0 && kNorm; off >>= 1) s.sum += __shfl_xor_sync(0xffffffffu, s.sum, off);
     if (lane == 0) {
-        warp_sum[warp] = sum;
-        warp_max[warp] = big;
-        warp_bad[warp] = bad;
+        warp_sum[warp] = s.sum;
+        warp_big[warp] = s.big_bits;
     }
     __syncthreads();
-    sum = 0.0f;
-    big = 0.0f;
-    int any_bad = 0;
+    s = {0.0f, 0u};
 #pragma unroll
     for (int w = 0; w < kQuantThreads / 32; ++w) {
-        sum += warp_sum[w];
-        big = fmaxf(big, warp_max[w]);
-        any_bad |= warp_bad[w];
+        s.sum += warp_sum[w];
+        s.big_bits = max(s.big_bits, warp_big[w]);
     }
-    QuantRow r;
-    r.pre = big > 1.0e30f ? 0x1p-64f : (big < 1.0e-30f ? 0x1p64f : 1.0f);
-    r.largest = big * r.pre;
-    const bool flat = !(big > 0.0f) || any_bad;           // nothing to quantise: every q is zero
-    r.ratio = flat ? 0.0f : 127.0f / r.largest;
-    if (tid == 0) {
-        float s = big / 127.0f;
-        if (norm_weight) s *= rsqrtf(sum / (float)dim + epsilon);
-        scale[blockIdx.x] = any_bad ? CUDART_NAN_F : s;
-    }
+    const QuantRow r = quant_row(s.big_bits);
+    if (tid == 0) scale[blockIdx.x] = row_scale(r, s.sum, kNorm, dim, epsilon);
     if (kVector) {
-        for (int v = tid; v < dim / 8; v += kQuantThreads) {
-            const uint4 raw = row_vectors[v];
-            uint4 wv = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
-            if (norm_weight) wv = __ldg(reinterpret_cast<const uint4*>(norm_weight + 8 * v));
-            const uint32_t* rw = reinterpret_cast<const uint32_t*>(&raw);
-            const uint32_t* ww = reinterpret_cast<const uint32_t*>(&wv);
-            uint32_t packed[2] = {0u, 0u};
-            if (!flat) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int lo = quantize_value(bf16_lo(rw[i]) * bf16_lo(ww[i]), r);
-                    const int hi = quantize_value(bf16_hi(rw[i]) * bf16_hi(ww[i]), r);
-                    packed[i >> 1] |= ((uint32_t)(lo & 0xff) | ((uint32_t)(hi & 0xff) << 8)) << (16 * (i & 1));
-                }
-            }
-            *reinterpret_cast<uint2*>(q + base + 8 * v) = make_uint2(packed[0], packed[1]);
-        }
+        for (int v = tid; v < dim / 8; v += kQuantThreads)
+            *reinterpret_cast<uint2*>(q + base + 8 * v) = quantize_eight<kNorm>(row_vectors[v], kNorm ? __ldg(weights + v) : none, r);
     } else {
         for (int c = tid; c < dim; c += kQuantThreads) {
-            const float w = norm_weight ? bf16_bits_to_f32(norm_weight[c]) : 1.0f;
-            q[base + c] = flat ? (int8_t)0 : (int8_t)quantize_value(bf16_bits_to_f32(staged[c]) * w, r);
+            const float w = kNorm ? bf16_bits_to_f32(norm_weight[c]) : 1.0f;
+            q[base + c] = r.flat ? (int8_t)0 : (int8_t)quantize_exactly(bf16_bits_to_f32(staged[c]) * w, r);
         }
     }
 }
+
+// A warp per row: many rows.  Nothing but shuffles between the two sweeps, the second of which finds the row in L1.
+template <bool kNorm>
+__global__ void __launch_bounds__(kQuantWarps * 32) qm_quantize_many_rows_kernel(const uint16_t* __restrict__ x,
+                                                                                const uint16_t* __restrict__ norm_weight,
+                                                                                float epsilon, int8_t* __restrict__ q,
+                                                                                float* __restrict__ scale, int dim, int rows) {
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const int row = blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const uint4* src = reinterpret_cast<const uint4*>(x + (size_t)row * dim);
+    const uint4* weights = reinterpret_cast<const uint4*>(norm_weight);
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+    const int vectors = dim / 8;
+    RowSweep s = {0.0f, 0u};
+#pragma unroll 8
+    for (int v = lane; v < vectors; v += 32) sweep_eight<kNorm>(src[v], kNorm ? __ldg(weights + v) : none, s);
+    s.big_bits = __reduce_max_sync(0xffffffffu, s.big_bits);
+#pragma unroll
+    for (int off = 16; off > 0 && kNorm; off >>= 1) s.sum += __shfl_xor_sync(0xffffffffu, s.sum, off);
+    const QuantRow r = quant_row(s.big_bits);
+    if (lane == 0) scale[row] = row_scale(r, s.sum, kNorm, dim, epsilon);
+    uint2* dst = reinterpret_cast<uint2*>(q + (size_t)row * dim);
+#pragma unroll 4
+    for (int v = lane; v < vectors; v += 32) dst[v] = quantize_eight<kNorm>(src[v], kNorm ? __ldg(weights + v) : none, r);
+}
+// Measured with the norm, us, a CTA per row / a warp per row: 2048 columns, 2048 rows 6.5 / 7.5, 9923 rows 24.1 / 19.2;
+// 4096 columns, 16384 rows 71.6 / 74.9; 6144 columns, 9923 rows 60.3 / 76.4.
+constexpr int kManyRows = 4096, kManyRowsDim = 2048;
 
 // ---- shared by the two products -----------------------------------------------------------------------------------
 
@@ -149,8 +212,9 @@ constexpr int kChunk = 128;                    // K columns (bytes) per ring sta
 constexpr int kSkinnyThreads = 192;            // warps 0-3 epilogue, warp 4 MMA issue, warp 5 TMA
 constexpr int kWeightRows = 128;
 
-// gate * sigmoid(gate) * up in fp32
-__device__ __forceinline__ float gated(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
+// gate * sigmoid(gate) * up in fp32; the fast division is within 2 units in the last place (and gives 0 below a gate of
+// -87, where the product is under 1e-36 of up)
+__device__ __forceinline__ float gated(float gate, float up) { return __fdividef(gate, 1.0f + __expf(-gate)) * up; }
 
 // The copying thread sees its last copies land (bounded) before it leaves, so that none is in flight into the shared
 // memory of a CTA that has retired after some other thread's wait gave up.
@@ -259,6 +323,20 @@ qm_skinny_int8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_co
     bool dead = false;
     pdl_wait();
 
+    constexpr int kGroups = kGated ? 16 : 32;              // pieces of four columns in a tile
+    const int n_cols = a.out_cols[seg];
+    const int g = tid % kGroups;
+    const int col = (kGated ? tile * 64 : tile * kWeightRows) + 4 * g;
+    float sw[4], extra[4];                                 // column scales; the up scales (gated) or the bias
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool in = warp < 4 && col + i < n_cols;
+        sw[i] = in ? a.w_scale[seg][col + i] : 0.0f;
+        extra[i] = 0.0f;
+        if (kGated) extra[i] = in ? a.w_scale[1][col + i] : 0.0f;
+        else if (in && a.bias[seg]) extra[i] = bf16_bits_to_f32(a.bias[seg][col + i]);
+    }
+
     if (warp == 5) {
         if (lane == 0) {
             const uint64_t weights_once = l2_policy_evict_first();
@@ -318,45 +396,43 @@ qm_skinny_int8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_co
     cluster_sync_all();
 
     if (warp < 4) {
-        // rank r finishes the token rows r, r + split, ...; a work item is one of them x four weight rows
+        // Rank r finishes the token rows r, r + split, ...; a thread keeps its four neighbouring weight rows of the tile
+        // (whose scales and bias it fetched before the sums were ready) and walks those token rows.  All loads of a step
+        // are issued before the first is used.
         const uint32_t reduce_addr = sbase + L::kReduce;
-        constexpr int kGroups = kGated ? 16 : 32;
         uint32_t peer[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) peer[k] = map_to_rank(reduce_addr, (uint32_t)(k < a.split ? k : 0));
-        const int owned = ((int)rank < a.rows) ? (a.rows - 1 - (int)rank) / a.split + 1 : 0;
-        const int n_cols = a.out_cols[seg];
-        for (int item = tid; item < owned * kGroups; item += 128) {
-            const int g = item % kGroups;
-            const int m = (int)rank + (item / kGroups) * a.split;
+        for (int m = (int)rank + (tid / kGroups) * a.split; m < a.rows; m += (128 / kGroups) * a.split) {
             const uint32_t off = (uint32_t)(m * kWeightRows + 4 * g) * 4u;
+            const size_t o = (size_t)m * n_cols + col;
+            const float sx = a.x_scale[m];
+            float res[4] = {0.f, 0.f, 0.f, 0.f};
+            if (!kGated && a.residual) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (col + i < n_cols) res[i] = bf16_bits_to_f32(a.residual[o + i]);
+            }
+            int4 part[8], part2[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                part[k] = part2[k] = make_int4(0, 0, 0, 0);
+                if (k < a.split) {
+                    part[k] = ld_cluster_s32x4(peer[k] + off);
+                    if (kGated) part2[k] = ld_cluster_s32x4(peer[k] + off + 64u * 4u);
+                }
+            }
             int acc[4] = {0, 0, 0, 0}, acc2[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                if (k >= a.split) break;
-                const int4 p = ld_cluster_s32x4(peer[k] + off);
-                acc[0] += p.x; acc[1] += p.y; acc[2] += p.z; acc[3] += p.w;
-                if (kGated) {
-                    const int4 p2 = ld_cluster_s32x4(peer[k] + off + 64u * 4u);
-                    acc2[0] += p2.x; acc2[1] += p2.y; acc2[2] += p2.z; acc2[3] += p2.w;
-                }
+                acc[0] += part[k].x; acc[1] += part[k].y; acc[2] += part[k].z; acc[3] += part[k].w;
+                acc2[0] += part2[k].x; acc2[1] += part2[k].y; acc2[2] += part2[k].z; acc2[3] += part2[k].w;
             }
-            const int col = (kGated ? tile * 64 : tile * kWeightRows) + 4 * g;
-            const size_t o = (size_t)m * n_cols + col;
-            const float sx = a.x_scale[m];
             uint32_t bits[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                bits[i] = 0u;
-                if (col + i >= n_cols) continue;
-                float v = (float)acc[i] * sx * __ldg(a.w_scale[seg] + col + i);
-                if (kGated) {
-                    v = gated(v, (float)acc2[i] * sx * __ldg(a.w_scale[1] + col + i));
-                } else {
-                    if (a.bias[seg]) v += bf16_bits_to_f32(__ldg(a.bias[seg] + col + i));
-                    if (a.residual) v += bf16_bits_to_f32(a.residual[o + i]);
-                }
-                bits[i] = f32_to_bf16_bits(v);
+                const float v = (float)acc[i] * sx * sw[i];
+                bits[i] = f32_to_bf16_bits(kGated ? gated(v, (float)acc2[i] * sx * extra[i]) : v + extra[i] + res[i]);
             }
             uint16_t* dst = a.out[seg] + o;
             if (col + 3 < n_cols && (reinterpret_cast<uintptr_t>(dst) & 7u) == 0) {
@@ -639,19 +715,37 @@ struct Int8Segment {
     int out_cols;
 };
 
-// CTAs that share a tile's K range: enough of them for two per SM, a power of two up to 8, two chunks each at least.
+// CTAs that share a tile's K range, a power of two up to 8: doubled while that stays within two CTAs per SM and leaves
+// each at least two chunks, or four where it would put a second CTA on SMs.  Measured, us, at 2048 -> 4096 (32 tiles, 16
+// chunks) for 1 / 32 / 64 rows: split 2 6.0 / 7.5 / 9.4, split 4 5.0 / 5.8 / 6.9, split 8 5.1 / 6.5 / 7.7; at 4096 -> 4096
+// (32 chunks) split 4 7.0 / 8.1 / 9.2, split 8 6.5 / 7.8 / 8.9.
 int int8_split(int tiles, int chunks, int sms) {
     int split = 1;
-    while (split < 8 && tiles * split * 2 <= 2 * sms && chunks / (split * 2) >= 2) split *= 2;
+    while (split < 8) {
+        const int next = 2 * split;
+        if (tiles * next > 2 * sms || chunks / next < (tiles * next > sms ? 4 : 2)) break;
+        split = next;
+    }
     return split;
 }
 
+// The opt-in to a kernel's shared memory, once per thread and device.
+template <typename Kernel>
+int32_t allow_smem(Kernel kernel, size_t bytes, int device, int& known_device, const char* what) {
+    if (known_device == device) return QM_OK;
+    QM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what);
+    known_device = device;
+    return QM_OK;
+}
+
 template <int kMPad, bool kGated>
-int32_t launch_skinny(const CUtensorMap* maps, const CUtensorMap& x_map, const Int8Args& a, unsigned grid, cudaStream_t stream,
-                      const char* what) {
+int32_t launch_skinny(const CUtensorMap* maps, const CUtensorMap& x_map, const Int8Args& a, unsigned grid, int device,
+                      cudaStream_t stream, const char* what) {
     auto kernel = qm_skinny_int8_kernel<kMPad, kGated>;
     const size_t smem = SkinnySmem<kMPad>::kTotal + 1024;
-    QM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), what);
+    static thread_local int known_device = -1;
+    const int32_t rc = allow_smem(kernel, smem, device, known_device, what);
+    if (rc != QM_OK) return rc;
     QM_CUDA_TRY(launch_cluster(kernel, dim3(grid), dim3(kSkinnyThreads), (unsigned)a.split, smem, stream, maps[0], maps[1],
                                maps[2], x_map, a),
                 what);
@@ -659,7 +753,8 @@ int32_t launch_skinny(const CUtensorMap* maps, const CUtensorMap& x_map, const I
 }
 
 template <int kBN, bool kGated>
-int32_t launch_rows(const int8_t* x, const int8_t* w0, const int8_t* w1, Int8Args& a, int sms, cudaStream_t stream, const char* what) {
+int32_t launch_rows(const int8_t* x, const int8_t* w0, const int8_t* w1, Int8Args& a, int sms, int device, cudaStream_t stream,
+                    const char* what) {
     constexpr int kCols = kGated ? kBN / 2 : kBN;
     CUtensorMap x_map, w0_map, w1_map, out_map{};
     int32_t rc = encode_byte_map(&x_map, x, (uint64_t)a.rows, (uint64_t)a.k_dim, 128);
@@ -672,7 +767,9 @@ int32_t launch_rows(const int8_t* x, const int8_t* w0, const int8_t* w1, Int8Arg
     if (tiles > 0x7fffffffLL) return qm_fail(QM_ECAPACITY, "too many output tiles for one launch");
     auto kernel = qm_rows_int8_kernel<kBN, kGated>;
     const size_t smem = RowsSmem<kBN>::kTotal + 1024;
-    QM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), what);
+    static thread_local int known_device = -1;
+    rc = allow_smem(kernel, smem, device, known_device, what);
+    if (rc != QM_OK) return rc;
     QM_CUDA_TRY(qm_launch(kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(kRowsThreads), smem, stream, x_map, w0_map,
                           w1_map, out_map, a),
                 what);
@@ -721,6 +818,10 @@ int32_t run_int8(qm_kv_pool* pool, const int8_t* x, const float* x_scale, const 
             a.weight[i] = second ? up : sg.weight;
             a.w_scale[i] = second ? up_scale : sg.scale;
             a.first_tile[i] = i < n_segs ? tiles : 0x7fffffff;
+            if (i >= n_segs && !second) {          // unused: any valid map will do
+                maps[i] = maps[i - 1];
+                continue;
+            }
             const int32_t rc = encode_byte_map(&maps[i], a.weight[i], (uint64_t)sg.out_cols, (uint64_t)k_dim, (uint32_t)rows_per_tile);
             if (rc != QM_OK) return rc;
             if (i < n_segs) {
@@ -735,9 +836,9 @@ int32_t run_int8(qm_kv_pool* pool, const int8_t* x, const float* x_scale, const 
         if (rc != QM_OK) return rc;
         a.split = int8_split(tiles, a.chunks, sms);
         const unsigned grid = (unsigned)tiles * (unsigned)a.split;
-        if (m_pad == 16) return launch_skinny<16, kGated>(maps, x_map, a, grid, stream, what);
-        if (m_pad == 32) return launch_skinny<32, kGated>(maps, x_map, a, grid, stream, what);
-        return launch_skinny<64, kGated>(maps, x_map, a, grid, stream, what);
+        if (m_pad == 16) return launch_skinny<16, kGated>(maps, x_map, a, grid, device, stream, what);
+        if (m_pad == 32) return launch_skinny<32, kGated>(maps, x_map, a, grid, device, stream, what);
+        return launch_skinny<64, kGated>(maps, x_map, a, grid, device, stream, what);
     }
     a.m_tiles = (rows + 127) / 128;
     for (int i = 0; i < n_segs; ++i) {
@@ -754,9 +855,9 @@ int32_t run_int8(qm_kv_pool* pool, const int8_t* x, const float* x_scale, const 
         };
         const int8_t* second = kGated ? up : segs[i].weight;
         int32_t rc;
-        if (enough(256)) rc = launch_rows<256, kGated>(x, segs[i].weight, second, a, sms, stream, what);
-        else if (enough(128)) rc = launch_rows<128, kGated>(x, segs[i].weight, second, a, sms, stream, what);
-        else rc = launch_rows<64, kGated>(x, segs[i].weight, second, a, sms, stream, what);
+        if (enough(256)) rc = launch_rows<256, kGated>(x, segs[i].weight, second, a, sms, device, stream, what);
+        else if (enough(128)) rc = launch_rows<128, kGated>(x, segs[i].weight, second, a, sms, device, stream, what);
+        else rc = launch_rows<64, kGated>(x, segs[i].weight, second, a, sms, device, stream, what);
         if (rc != QM_OK) return rc;
     }
     return QM_OK;
@@ -775,12 +876,20 @@ int32_t qm_quantize_rows_int8(const uint16_t* x, const uint16_t* norm_weight, fl
     if ((bf16s & 1u) || (reinterpret_cast<uintptr_t>(scale) & 3u)) return qm_fail(QM_EINVAL, "misaligned tensor pointer");
     const size_t smem = ((size_t)dim * 2 + 15) / 16 * 16;
     const bool vector = dim % 8 == 0 && (bf16s & 15u) == 0 && (reinterpret_cast<uintptr_t>(q) & 7u) == 0;
-    auto kernel = vector ? qm_quantize_rows_kernel<true> : qm_quantize_rows_kernel<false>;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (vector && rows >= kManyRows && dim <= kManyRowsDim) {
+        const dim3 grid((unsigned)((rows + kQuantWarps - 1) / kQuantWarps));
+        QM_CUDA_TRY(qm_launch(norm_weight ? qm_quantize_many_rows_kernel<true> : qm_quantize_many_rows_kernel<false>, grid,
+                              dim3(kQuantWarps * 32), 0, s, x, norm_weight, epsilon, q, scale, (int)dim, (int)rows),
+                    "row quantisation launch");
+        return QM_OK;
+    }
+    auto kernel = vector ? (norm_weight ? qm_quantize_rows_kernel<true, true> : qm_quantize_rows_kernel<true, false>)
+                         : (norm_weight ? qm_quantize_rows_kernel<false, true> : qm_quantize_rows_kernel<false, false>);
     if (smem > 47 * 1024)         // the row and the static words together pass the 48 KB that need no opt-in
         QM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kQuantMaxDim * 2),
                     "raise row quantisation shared memory");
-    QM_CUDA_TRY(qm_launch(kernel, dim3((unsigned)rows), dim3(kQuantThreads), smem, static_cast<cudaStream_t>(stream), x, norm_weight,
-                          epsilon, q, scale, (int)dim),
+    QM_CUDA_TRY(qm_launch(kernel, dim3((unsigned)rows), dim3(kQuantThreads), smem, s, x, norm_weight, epsilon, q, scale, (int)dim),
                 "row quantisation launch");
     return QM_OK;
 }

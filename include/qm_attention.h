@@ -467,6 +467,29 @@ int32_t qm_final_head_sample(qm_kv_pool* pool, const uint16_t* logits, int32_t b
                              int32_t eos_token, int32_t reserved_begin, int32_t top_k, float temperature,
                              uint64_t* rng_state, int32_t* codes_out, float* processed_out, void* stream);
 
+/* Sampling from given uniform numbers, every row with parameters of its own.  The reference draws from at most 4096
+ * codes with top-k only and its own generator (gpu_sample_topk_f32_kernel, 17.cu:7546; qm_final_head_sample here);
+ * the processed scores that qm_final_head_sample writes can be the logits of this call.
+ * For a row z with temperature T > 0: w_i = exp((z_i - max z) / T), order = z descending, index ascending among equals.
+ *   top_k  (> 0)     keeps the first top_k entries of that order
+ *   top_p  (< 1)     keeps, of those, each entry whose predecessors' weights sum to less than top_p times the sum of
+ *                    all of them; the first entry always stays
+ *   min_p  (> 0)     keeps, of those, the entries with w_i >= min_p; the largest scores always stay
+ *   draw             the lowest index i at which the kept weights up to and including w_i, in index order, exceed
+ *                    uniforms[row] times their sum (uniforms in [0, 1); anything below is 0, anything above picks the
+ *                    last kept entry)
+ * T <= 0 (or NaN) picks the first entry of the order.  NaN scores are never drawn; -inf is a weight of zero; a row
+ * without any score above -inf gives token -1 and probability 0.  Weights are exact to about 1e-14 of the largest
+ * and their sums do not depend on timing: the same inputs give the same tokens.
+ *   logits: row r at element r * row_stride (0: one row, many draws), bf16, or fp32 with logits_are_fp32 != 0; vocab from
+ *   1 to 262144, no alignment needed beyond the element's
+ *   temperature, top_k, top_p, min_p [batch]: each may be NULL (1, off, off, off)
+ *   probs_out [batch] (or NULL): the token's weight over the sum of the kept weights; 1 where T <= 0
+ * The current device must be the one that holds the tensors. */
+int32_t qm_sample_filtered(const void* logits, int32_t logits_are_fp32, int64_t row_stride, int32_t batch, int32_t vocab,
+                           const float* uniforms, const float* temperature, const int32_t* top_k, const float* top_p,
+                           const float* min_p, int32_t* tokens_out, float* probs_out, void* stream);
+
 /* gather_embedding_kernel (17.cu:8875-8893) for a batch of rows: out[r][:] = table[token_ids[r]][:].
  * table [vocab][hidden] bf16, hidden a multiple of 8; an id outside the table is clamped and reported in the
  * pool's status word (QM_DEVSTAT_BAD_POS). */

@@ -91,6 +91,7 @@ ABI = {
     "qm_gate_up_swiglu_int8": (c_int32, [c_void_p] * 8 + [c_int32, c_int32, c_int32, c_void_p]),
     "qm_final_head_sample": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_int32, c_int32,
                                        c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "qm_sample_filtered": (c_int32, [c_void_p, c_int32, c_int64, c_int32, c_int32] + [c_void_p] * 8),
     "qm_embedding_gather": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
     "qm_exchange_buffer_bytes": (c_int64, [c_int32, c_int32]),
     "qm_attention_exchange_combine": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32,
@@ -481,6 +482,28 @@ class TalkerAttention:
                                              _ptr(generation_index), flags, eos_token, reserved_begin, top_k,
                                              float(temperature), _ptr(rng_state), _ptr(codes), _ptr(processed), _stream()))
         return codes
+
+    def sample_filtered(self, logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, probs=None):
+        """Temperature, top-k, top-p, min-p and the draw from given uniform numbers; every parameter is a tensor with one
+        value per row, or None.  logits [batch][vocab] bf16 or fp32, rows at any stride.  Returns (tokens, probabilities
+        of the tokens among what the filters left)."""
+        import torch
+
+        batch, vocab = logits.shape
+        if logits.dtype not in (torch.bfloat16, torch.float32) or not logits.is_cuda or (vocab > 1 and logits.stride(1) != 1):
+            raise ValueError("logits: expected CUDA rows of bfloat16 or float32 without gaps between their elements")
+        tokens = logits.new_empty((batch,), dtype=torch.int32) if tokens is None else tokens
+        probs = logits.new_empty((batch,), dtype=torch.float32) if probs is None else probs
+        _packed(torch.float32, uniforms, temperature, top_p, min_p, probs)
+        _packed(torch.int32, top_k, tokens)
+        for what, t in (("uniforms", uniforms), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p),
+                        ("tokens", tokens), ("probs", probs)):
+            _shaped(what, t, batch)
+        stride = logits.stride(0) if batch > 1 else vocab
+        _check(self.lib.qm_sample_filtered(_ptr(logits), int(logits.dtype == torch.float32), stride, batch, vocab, _ptr(uniforms),
+                                           _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(tokens), _ptr(probs),
+                                           _stream()))
+        return tokens, probs
 
     def embedding_gather(self, table, token_ids, out=None):
         """gather_embedding_kernel (17.cu:8875) for a batch: out[r] = table[token_ids[r]]."""

@@ -223,7 +223,30 @@ int32_t qm_decode_attention_static(qm_kv_pool* pool, int32_t layer, const uint16
  * call that reported QM_DEVSTAT_TIMEOUT; the pool's device must be current. */
 int32_t qm_decode_static_scratch_reset(qm_kv_pool* pool, void* stream);
 
-/* Same, but stops before normalisation and returns the partial softmax state
+/* The same attention for streams that share a long prefix (many requests behind one voice prompt), the shared keys read
+ * once per 64 streams instead of once per stream.  No counterpart in the reference (one stream; launch_attention with
+ * query_length 1, 17.cu:17895).  Arguments and result are those of qm_decode_attention (a row may differ from it in
+ * its last bf16 bits: the shared part runs on the tensor cores, its softmax weights rounded to bf16), and
+ *   group_starts [groups + 1], shared_pages [groups]: streams group_starts[g] .. group_starts[g + 1] - 1 have the same first
+ *     shared_pages[g] entries in their rows of page_table.  Nothing is copied or marked: those pages hold ordinary
+ *     tokens, written by whichever stream was prefilled first, and a prefix that ends inside a page shares the pages in
+ *     front of that one.
+ *   max_shared_pages: at least the largest of shared_pages, as known to the host (larger entries are cut to it)
+ * The entries need only agree among the group's streams that are at least shared_pages[g] * 64 keys long; a shorter
+ * stream is attended on its own, as is one outside all groups.  group_starts that decrease or leave 0 .. batch are
+ * forced into order and set QM_DEVSTAT_BAD_POS.
+ * At most 256 streams and 256 groups per call (QM_ECAPACITY).  `workspace`: qm_decode_shared_workspace_bytes(pool, batch)
+ * bytes, 16-byte aligned, prepared once with qm_decode_workspace_init, and not shared by calls that overlap on the GPU
+ * (it serves qm_decode_attention too, in turn).  The pool's device must be the current device.
+ * Deterministic: the pieces depend on the lengths, the groups and the SM count, and are folded in order. */
+int64_t qm_decode_shared_workspace_bytes(const qm_kv_pool* pool, int32_t batch);
+int32_t qm_decode_attention_shared(qm_kv_pool* pool, int32_t layer, const uint16_t* q_rot, const int32_t* seq_lens,
+                                   const int32_t* page_table, int32_t max_pages, int32_t batch, int32_t q_heads,
+                                   const int32_t* group_starts, const int32_t* shared_pages, int32_t groups,
+                                   int32_t max_shared_pages, uint16_t* out, void* workspace, int64_t workspace_bytes,
+                                   void* stream);
+
+/* qm_decode_attention again, but it stops before normalisation and returns the partial softmax state
  * of each (stream, query head) over the keys held in THIS pool:
  *   partial [batch][q_heads][130] fp32 = { m (max scaled score, natural-log
  *   domain), l (sum of exp(s - m)), o[128] (unnormalised) }.

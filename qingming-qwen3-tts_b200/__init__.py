@@ -75,6 +75,9 @@ ABI = {
                                                                     c_float, c_void_p, c_void_p, c_int64, c_void_p]),
     "qm_decode_attention_static": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
                                              c_int32, c_void_p, c_void_p]),
+    "qm_decode_shared_workspace_bytes": (c_int64, [c_void_p, c_int32]),
+    "qm_decode_attention_shared": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,
+                                             c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_int64, c_void_p]),
     "qm_decode_attention_partial": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_int32,
                                               c_int32, c_void_p, c_void_p, c_int64, c_void_p]),
     "qm_attention_combine": (c_int32, [c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
@@ -203,6 +206,7 @@ class TalkerAttention:
         self.rope_sin = torch.empty_like(self.rope_cos)
         _check(self.lib.qm_rope_table_fill(_ptr(self.rope_cos), _ptr(self.rope_sin), max_positions, 0, theta, _stream()))
         self._workspace = None
+        self._shared_workspace = None
 
     def close(self) -> None:
         if getattr(self, "pool", None):
@@ -299,6 +303,31 @@ class TalkerAttention:
         _check(self.lib.qm_decode_attention(self.pool, layer, _ptr(q_rot), _ptr(seq_lens), _ptr(page_table),
                                             page_table.shape[1], batch, self.q_heads, _ptr(out), _ptr(ws),
                                             ws.numel(), _stream()))
+        return out
+
+    def launch_attention_shared(self, layer, q_rot, seq_lens, page_table, group_starts, shared_pages, max_shared_pages, out=None):
+        """Decode attention for groups of streams whose tables begin with the same pages: streams group_starts[g] ..
+        group_starts[g + 1] - 1 share their first shared_pages[g] pages, which are read once for all of them."""
+        import torch
+
+        batch, groups = q_rot.shape[0], shared_pages.shape[0]
+        out = torch.empty_like(q_rot) if out is None else out
+        _packed(torch.bfloat16, q_rot, out)
+        _packed(torch.int32, seq_lens, page_table, group_starts, shared_pages)
+        _shaped("q_rot", q_rot, batch, self.q_heads, HEAD_DIM)
+        _shaped("out", out, batch, self.q_heads, HEAD_DIM)
+        _shaped("seq_lens", seq_lens, batch)
+        _shaped("page_table", page_table, batch, page_table.shape[1])
+        _shaped("group_starts", group_starts, groups + 1)
+        ws = self._shared_workspace
+        if ws is None or self._shared_batch < batch:
+            need = self.lib.qm_decode_shared_workspace_bytes(self.pool, batch)
+            self._shared_workspace = ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+            self._shared_batch = batch
+            _check(self.lib.qm_decode_workspace_init(_ptr(ws), need, _stream()))
+        _check(self.lib.qm_decode_attention_shared(
+            self.pool, layer, _ptr(q_rot), _ptr(seq_lens), _ptr(page_table), page_table.shape[1], batch, self.q_heads,
+            _ptr(group_starts), _ptr(shared_pages), groups, max_shared_pages, _ptr(out), _ptr(ws), ws.numel(), _stream()))
         return out
 
     def decode_step(self, layer, q, k, v, q_norm_weight, k_norm_weight, positions, page_table, out=None):

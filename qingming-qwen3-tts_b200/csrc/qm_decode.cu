@@ -31,6 +31,7 @@
 
 #include "qm_exchange_layout.cuh"
 #include "qm_norm_rope.cuh"
+#include "qm_shared_groups.cuh"
 
 namespace {
 
@@ -77,6 +78,7 @@ struct DecodeArgs {
                              //    the other ranks' and folded here (keys split across GPUs), bf16 context
     int prefetch_units;      // units per CTA whose tiles are prefetched into L2 before the dependency wait
     ExchangeView exchange;   // mode 2: every rank's exchange buffer
+    SharedGroups shared;     // kShared: groups of streams whose first pages another kernel has attended
 };
 
 struct SharedLayout {
@@ -94,7 +96,11 @@ struct SharedLayout {
     static constexpr int kExchangeOff = kFlagOff + 16;           // uint32[2][2]: per query head, for the fused exchange
     static constexpr int kPeerOff = kExchangeOff + 16;           // the ranks' exchange buffer pointers (mode 2)
     static constexpr int kTotal = kPeerOff + kExchangeMaxWorld * 8;
+    // shared prefixes only: the first page each stream attends here
+    static constexpr int kFirstPageOff = kTotal;
+    static constexpr int kTotalShared = kFirstPageOff + kMaxBatchPerLaunch * 2;
 };
+static_assert((kMaxBatchPerLaunch + 1) * 4 <= kConsumerWarps * 2 * kHeadDim * 4, "group boundaries fit where warps merge later");
 
 __device__ __forceinline__ int clamp_len(int len, int max_pages, uint32_t* status) {
     if (len < 0) len = 0;
@@ -106,7 +112,10 @@ __device__ __forceinline__ int clamp_len(int len, int max_pages, uint32_t* statu
     return len;
 }
 
-template <bool kFused, bool kExchange = false>
+// kShared: the streams' first pages have been attended by the launch in front (qm_shared_prefix.cu), which lets this one
+// start only after everything in front of IT is complete.  So lengths, tables, queries and K/V are read without a
+// wait, the two launches overlap, and only the fold of the other one's partial results waits for it.
+template <bool kFused, bool kExchange = false, bool kShared = false>
 __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(const DecodeArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     int32_t* prefix = reinterpret_cast<int32_t*>(smem + SharedLayout::kPrefixOff);
@@ -148,7 +157,12 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
     // again in any case.  Only if a length changed is the partition rebuilt.  A wrong guess costs a useless
     // prefetch and nothing else.
     const int cap_len = a.max_pages * kPageTokens;
-    auto units_of = [&](int len) { return ((len + kPageTokens - 1) >> 6) * hkv; };
+    uint16_t* first_page = reinterpret_cast<uint16_t*>(smem + SharedLayout::kFirstPageOff);       // kShared
+    auto units_of = [&](int len) {
+        int pages = (len + kPageTokens - 1) >> 6;
+        if (kShared) pages = pages > (int)first_page[tid] ? pages - (int)first_page[tid] : 0;
+        return pages * hkv;
+    };
     // prefix[s + 1] holds the units of stream s on entry; on exit prefix[s] = first unit of stream s
     auto scan_prefix = [&]() {
         __syncthreads();
@@ -187,9 +201,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
         um.page_idx = r - um.head * um.pages;
         um.seg = lo * hkv + um.head;
         um.len = stream_len[lo];
-        const int left = um.len - um.page_idx * kPageTokens;
+        const int table_page = um.page_idx + (kShared ? (int)first_page[lo] : 0);
+        const int left = um.len - table_page * kPageTokens;
         um.nvalid = left < kPageTokens ? left : kPageTokens;
-        um.table_index = (long long)lo * a.max_pages + um.page_idx;
+        um.table_index = (long long)lo * a.max_pages + table_page;
         return um;
     };
 
@@ -233,7 +248,18 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
             }
         }
     }
-    pdl_wait();      // everything below reads what earlier kernels on the stream wrote
+    if (kShared) {
+        int* starts = reinterpret_cast<int*>(merge_o);
+        if (warp == 0) load_group_starts(a.shared, a.batch, starts, a.status, lane);
+        __syncthreads();
+        if (tid < a.batch) {
+            const int group = group_of_stream(starts, a.shared.groups, tid);
+            const int len = a.seq_lens[tid];
+            first_page[tid] = (uint16_t)(group < 0 ? 0 : shared_pages_of(a.shared, group, len < cap_len ? len : cap_len));
+        }
+    } else {
+        pdl_wait();      // everything below reads what earlier kernels on the stream wrote
+    }
 
     // The lengths as they are now (one per thread: a launch takes at most kMaxBatchPerLaunch <= blockDim streams).
     int my_len = 0;
@@ -261,6 +287,22 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
         xview = exchange_cache_peers(a.exchange, reinterpret_cast<unsigned char**>(smem + SharedLayout::kPeerOff), tid);
         __syncthreads();
     }
+    // Behind shared pages a stream without keys of its own still has the shared ones: those rows are written at the
+    // end, when the other launch's results are there.
+    auto write_streams_without_units = [&]() {
+        pdl_wait();
+        for (int s = blockIdx.x; s < a.batch; s += gridDim.x) {
+            if (prefix[s + 1] != prefix[s]) continue;
+            const int4 words = __ldcg(reinterpret_cast<const int4*>(a.shared.streams + s));
+            const SharedStream st{words.x, words.y, words.z, words.w};
+            for (int i = tid; i < 2 * hkv * kHeadDim; i += kConsumerThreads) {
+                float m = -CUDART_INF_F, l = 0.0f, o = 0.0f;
+                fold_shared(a.shared, st, i / (2 * kHeadDim), (i / kHeadDim) & 1, i % kHeadDim, m, l, o);
+                a.out[(size_t)s * (2 * hkv) * kHeadDim + i] = l > 0.0f ? (uint16_t)f32_to_bf16_bits(o / l) : (uint16_t)0;
+            }
+        }
+    };
+    if constexpr (!kShared)
     for (int s = blockIdx.x; s < a.batch; s += gridDim.x) {
         if (prefix[s + 1] != prefix[s]) continue;
         if (kExchange) {
@@ -292,7 +334,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
     const long long total_units = prefix[a.batch];
     const long long grid_eff = total_units < (long long)gridDim.x ? total_units : (long long)gridDim.x;
     const int cta = blockIdx.x;
-    if (cta >= grid_eff) return;
+    if (cta >= grid_eff) {
+        if (kShared && warp < kConsumerWarps) write_streams_without_units();
+        return;
+    }
     const long long unit_begin = (long long)cta * total_units / grid_eff;
     const long long unit_end = (long long)(cta + 1) * total_units / grid_eff;
     const int count = (int)(unit_end - unit_begin);
@@ -607,6 +652,13 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
                 const float m = qh ? m1 : m0;
                 const bool whole = seg_from_start && page_idx == pages - 1;
                 const size_t row = (size_t)stream * (2 * hkv) + 2 * head + qh;
+                auto with_shared = [&](float m_own, float l_own, float o_own) {
+                    pdl_wait();
+                    const int4 words = __ldcg(reinterpret_cast<const int4*>(a.shared.streams + stream));
+                    const SharedStream st{words.x, words.y, words.z, words.w};
+                    fold_shared(a.shared, st, head, qh, d, m_own, l_own, o_own);
+                    return (uint16_t)f32_to_bf16_bits(o_own / l_own);
+                };
                 // `dead`: one of this thread's waits gave up (QM_DEVSTAT_TIMEOUT is set).  Its numbers are garbage
                 // and the unit description may be a stale one, so it writes nothing to global memory and takes
                 // no part in the arrival count; the barriers below are still passed by everyone.
@@ -616,6 +668,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
                         exchange_row(xview, (int)row, d, m * kLn2, lsum, sum, !dead, a.out + row * kHeadDim, a.status,
                                      exchange_words + 2 * qh, [qh] { if (qh) named_bar_sync(3, kHeadDim); else named_bar_sync(2, kHeadDim); });
                     } else if (dead) {
+                    } else if (kShared) {
+                        a.out[row * kHeadDim + d] = with_shared(m, lsum, sum);
                     } else if (a.mode == 0) {
                         a.out[row * kHeadDim + d] = (uint16_t)f32_to_bf16_bits(sum / lsum);
                     } else {
@@ -690,6 +744,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
                             exchange_row(xview, (int)row, d, big * kLn2, denom, acc, !dead, a.out + row * kHeadDim, a.status,
                                          exchange_words + 2 * qh, [qh] { if (qh) named_bar_sync(3, kHeadDim); else named_bar_sync(2, kHeadDim); });
                         } else if (dead) {
+                        } else if (kShared) {
+                            a.out[row * kHeadDim + d] = with_shared(big, denom, acc);
                         } else if (a.mode == 0) {
                             a.out[row * kHeadDim + d] = (uint16_t)f32_to_bf16_bits(acc / denom);
                         } else {
@@ -706,6 +762,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
             named_bar_sync(1, kConsumerThreads);
         }
     }
+    if (kShared) write_streams_without_units();
 }
 
 // ---------------------------------------------------------------------------
@@ -1075,6 +1132,41 @@ int32_t run_decode(qm_kv_pool* pool, int32_t layer, const uint16_t* q_rot, const
 }
 
 }  // namespace
+
+int32_t qm_launch_decode_behind_shared(qm_kv_pool* pool, int32_t layer, const uint16_t* q_rot, const int32_t* seq_lens,
+                                       const int32_t* page_table, int32_t max_pages, int32_t batch, uint16_t* out, void* workspace,
+                                       const SharedGroups& groups, cudaStream_t stream) {
+    static_assert(kSharedMaxBatch == kMaxBatchPerLaunch, "one launch");
+    static thread_local int attr_device = -1;
+    if (attr_device != pool->device) {
+        QM_CUDA_TRY(cudaFuncSetAttribute(qm_decode_splitkv_kernel<false, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         SharedLayout::kTotalShared),
+                    "raise decode kernel shared memory");
+        attr_device = pool->device;
+    }
+    int grid = 2 * pool->sm_count;
+    if (grid > kMaxGrid) grid = kMaxGrid;
+    unsigned char* ws = static_cast<unsigned char*>(workspace);
+    DecodeArgs a{};
+    a.q_rot = q_rot;
+    a.key_pool = qm_kv_pool_key_ptr(pool, layer);
+    a.value_pool = qm_kv_pool_value_ptr(pool, layer);
+    a.seq_lens = seq_lens;
+    a.page_table = page_table;
+    a.out = out;
+    a.ws_count = reinterpret_cast<int32_t*>(ws);
+    a.ws_partials = reinterpret_cast<float*>(ws + kCounterRegionBytes);
+    a.status = pool->status_dev;
+    a.batch = batch;
+    a.kv_heads = pool->kv_heads;
+    a.max_pages = max_pages;
+    a.num_pages = pool->num_pages;
+    a.shared = groups;
+    QM_CUDA_TRY(qm_launch(qm_decode_splitkv_kernel<false, false, true>, dim3(grid), dim3(kDecodeThreads), SharedLayout::kTotalShared,
+                          stream, a),
+                "split-KV decode attention behind shared pages launch");
+    return QM_OK;
+}
 
 extern "C" {
 

@@ -28,10 +28,11 @@
 
 #include <cstdlib>
 #include <mutex>
+#include <type_traits>
 
 #include "qm_exchange_layout.cuh"
 #include "qm_norm_rope.cuh"
-#include "qm_shared_groups.cuh"
+#include "qm_shared_prefix.cuh"
 
 namespace {
 
@@ -78,17 +79,18 @@ struct DecodeArgs {
                              //    the other ranks' and folded here (keys split across GPUs), bf16 context
     int prefetch_units;      // units per CTA whose tiles are prefetched into L2 before the dependency wait
     ExchangeView exchange;   // mode 2: every rank's exchange buffer
-    SharedGroups shared;     // kShared: groups of streams whose first pages another kernel has attended
+    SharedGroups shared;     // kShared: groups of streams that begin with the same pages (mode 1)
 };
 
-struct SharedLayout {
+template <int kStaging>
+struct DecodeLayout {
     static constexpr int kPrefixOff = kStages * kStageBytes;                       // int32[kMaxBatch+1]
     static constexpr int kLenOff = kPrefixOff + ((kMaxBatchPerLaunch + 1) * 4 + 15) / 16 * 16;   // int32[kMaxBatch]: keys per stream
     static constexpr int kScoreOff = kLenOff + kMaxBatchPerLaunch * 4;
     static constexpr int kMergeOff = kScoreOff + 2 * 2 * kPageTokens * 4;          // float[2][2][64]
     static constexpr int kMergeLOff = kMergeOff + kConsumerWarps * 2 * kHeadDim * 4;
-    // per stage: q rows of the two heads (512 B); fused step also cos, sin, raw k, raw v rows (256 B each)
-    static constexpr int kStagingBytes = 1536;
+    // per stage: q rows of the two heads (512 B); fused step (1536 B) also cos, sin, raw k, raw v rows (256 B each)
+    static constexpr int kStagingBytes = kStaging;
     static constexpr int kQOff = kMergeLOff + kConsumerWarps * 2 * 4;
     static constexpr int kMetaOff = kQOff + kStages * kStagingBytes;
     static constexpr int kBarOff = kMetaOff + kStages * 32;
@@ -96,11 +98,21 @@ struct SharedLayout {
     static constexpr int kExchangeOff = kFlagOff + 16;           // uint32[2][2]: per query head, for the fused exchange
     static constexpr int kPeerOff = kExchangeOff + 16;           // the ranks' exchange buffer pointers (mode 2)
     static constexpr int kTotal = kPeerOff + kExchangeMaxWorld * 8;
-    // shared prefixes only: the first page each stream attends here
-    static constexpr int kFirstPageOff = kTotal;
-    static constexpr int kTotalShared = kFirstPageOff + kMaxBatchPerLaunch * 2;
 };
-static_assert((kMaxBatchPerLaunch + 1) * 4 <= kConsumerWarps * 2 * kHeadDim * 4, "group boundaries fit where warps merge later");
+using SharedLayout = DecodeLayout<1536>;
+
+// kShared.  The ring holds the prefix role's tiles and starts on a 1024-byte boundary; the tables of the partition lie
+// where warps merge their results later.  The smaller staging areas (no fused step) keep two CTAs on an SM: measured, 114 712
+// bytes do and 115 224 do not, although the occupancy calculation says so.
+struct PrefixLayout : DecodeLayout<512> {
+    static constexpr int kFirstPageOff = kTotal;
+    static constexpr int kPrefixBarOff = kFirstPageOff + kMaxBatchPerLaunch * 2;
+    static constexpr int kTotalShared = kPrefixBarOff + kPrefixBars * 8 + 1024 - 128;
+};
+static_assert(SharedPlan::kBytes <= kConsumerWarps * 2 * kHeadDim * 4, "the partition's tables fit the merge area");
+static_assert(kPrefixTileBytes == kStages * kStageBytes, "the prefix role's tiles are the ring");
+static_assert(PrefixLayout::kPrefixBarOff % 8 == 0 && PrefixLayout::kMergeOff % 16 == 0, "alignment");
+static_assert(PrefixLayout::kTotalShared <= SharedLayout::kTotal, "two CTAs per SM");
 
 __device__ __forceinline__ int clamp_len(int len, int max_pages, uint32_t* status) {
     if (len < 0) len = 0;
@@ -112,20 +124,28 @@ __device__ __forceinline__ int clamp_len(int len, int max_pages, uint32_t* statu
     return len;
 }
 
-// kShared: the streams' first pages have been attended by the launch in front (qm_shared_prefix.cu), which lets this one
-// start only after everything in front of IT is complete.  So lengths, tables, queries and K/V are read without a
-// wait, the two launches overlap, and only the fold of the other one's partial results waits for it.
-template <bool kFused, bool kExchange = false, bool kShared = false>
-__global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(const DecodeArgs a) {
-    extern __shared__ __align__(128) unsigned char smem[];
-    int32_t* prefix = reinterpret_cast<int32_t*>(smem + SharedLayout::kPrefixOff);
-    int32_t* stream_len = reinterpret_cast<int32_t*>(smem + SharedLayout::kLenOff);
-    float* score = reinterpret_cast<float*>(smem + SharedLayout::kScoreOff);
-    float* merge_o = reinterpret_cast<float*>(smem + SharedLayout::kMergeOff);
-    float* merge_l = reinterpret_cast<float*>(smem + SharedLayout::kMergeLOff);
-    int4* meta = reinterpret_cast<int4*>(smem + SharedLayout::kMetaOff);      // two int4 per stage
-    volatile int* fold_flag = reinterpret_cast<volatile int*>(smem + SharedLayout::kFlagOff);
-    const uint32_t bar_base = smem_addr(smem + SharedLayout::kBarOff);
+// What only the variant with shared prefixes is given.
+struct NoMaps {};
+struct PrefixMaps {
+    CUtensorMap q, k, v;
+};
+
+// kShared: some of the CTAs attend the pages that groups of streams share (shared_prefix_role, qm_shared_prefix.cuh),
+// the others do what this kernel does in mode 1, over the pages behind those; how many of each is worked out here
+// from the lengths, so that both kinds have about the same number of pages and HBM is busy to the end.
+template <bool kFused, bool kExchange = false, bool kShared = false, typename Maps = NoMaps>
+__global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(const DecodeArgs a, const __grid_constant__ Maps maps) {
+    using L = std::conditional_t<kShared, PrefixLayout, SharedLayout>;
+    extern __shared__ __align__(128) unsigned char smem_base[];
+    unsigned char* smem = kShared ? smem_base + ((1024u - (smem_addr(smem_base) & 1023u)) & 1023u) : smem_base;
+    int32_t* prefix = reinterpret_cast<int32_t*>(smem + L::kPrefixOff);
+    int32_t* stream_len = reinterpret_cast<int32_t*>(smem + L::kLenOff);
+    float* score = reinterpret_cast<float*>(smem + L::kScoreOff);
+    float* merge_o = reinterpret_cast<float*>(smem + L::kMergeOff);
+    float* merge_l = reinterpret_cast<float*>(smem + L::kMergeLOff);
+    int4* meta = reinterpret_cast<int4*>(smem + L::kMetaOff);      // two int4 per stage
+    volatile int* fold_flag = reinterpret_cast<volatile int*>(smem + L::kFlagOff);
+    const uint32_t bar_base = smem_addr(smem + L::kBarOff);
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
     auto empty_bar = [&](int s) { return bar_base + 8u * (kStages + s); };
     auto staged_bar = [&](int s) { return bar_base + 8u * (2 * kStages + s); };
@@ -135,7 +155,15 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
     const int lane = tid & 31;
     const int hkv = a.kv_heads;
 
-    pdl_trigger();
+    // A kernel that can allocate TMEM holds the SM's right to do so from its start, and no second CTA starts beside it
+    // before it has given that up (measured: 148 CTAs at a time instead of 296, whether they allocate or not).  So every CTA
+    // allocates and relinquishes at once, and one without use for the columns frees them below.  The next launch is
+    // only let go after that: its CTAs may hold TMEM while they wait for this one.
+    if constexpr (kShared) {
+        if (warp == kPrefixTmemWarp) shared_prefix_tmem(smem_addr(smem + L::kFlagOff));
+    } else {
+        pdl_trigger();
+    }
     if (tid == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full_bar(s), kFused ? 2 : 1);       // producer (+ bytes) and, in the fused step, the prep warp
@@ -157,11 +185,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
     // again in any case.  Only if a length changed is the partition rebuilt.  A wrong guess costs a useless
     // prefetch and nothing else.
     const int cap_len = a.max_pages * kPageTokens;
-    uint16_t* first_page = reinterpret_cast<uint16_t*>(smem + SharedLayout::kFirstPageOff);       // kShared
+    uint16_t* first_page = reinterpret_cast<uint16_t*>(smem + PrefixLayout::kFirstPageOff);       // kShared
     auto units_of = [&](int len) {
-        int pages = (len + kPageTokens - 1) >> 6;
-        if (kShared) pages = pages > (int)first_page[tid] ? pages - (int)first_page[tid] : 0;
-        return pages * hkv;
+        const int pages = (len + kPageTokens - 1) >> 6;
+        return (kShared ? pages - (int)first_page[tid] : pages) * hkv;
     };
     // prefix[s + 1] holds the units of stream s on entry; on exit prefix[s] = first unit of stream s
     auto scan_prefix = [&]() {
@@ -201,14 +228,14 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
         um.page_idx = r - um.head * um.pages;
         um.seg = lo * hkv + um.head;
         um.len = stream_len[lo];
-        const int table_page = um.page_idx + (kShared ? (int)first_page[lo] : 0);
+        const int table_page = kShared ? um.page_idx + (int)first_page[lo] : um.page_idx;
         const int left = um.len - table_page * kPageTokens;
         um.nvalid = left < kPageTokens ? left : kPageTokens;
         um.table_index = (long long)lo * a.max_pages + table_page;
         return um;
     };
 
-    const bool speculate = a.prefetch_units > 0;
+    const bool speculate = !kShared && a.prefetch_units > 0;
     UnitMeta first_units{};                      // producer warp: lane l holds this CTA's unit l (speculated)
     bool first_units_known = false;
     if (speculate) {
@@ -248,17 +275,23 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
             }
         }
     }
-    if (kShared) {
-        int* starts = reinterpret_cast<int*>(merge_o);
-        if (warp == 0) load_group_starts(a.shared, a.batch, starts, a.status, lane);
-        __syncthreads();
-        if (tid < a.batch) {
-            const int group = group_of_stream(starts, a.shared.groups, tid);
-            const int len = a.seq_lens[tid];
-            first_page[tid] = (uint16_t)(group < 0 ? 0 : shared_pages_of(a.shared, group, len < cap_len ? len : cap_len));
+    pdl_wait();      // everything below reads what earlier kernels on the stream wrote
+
+    int cta = blockIdx.x, ctas = gridDim.x;
+    if constexpr (kShared) {
+        const SharedPlan plan = make_shared_plan(a.shared, a.seq_lens, a.batch, hkv, a.max_pages, (int)gridDim.x,
+                                                 smem + L::kMergeOff, first_page, a.status, tid, kDecodeThreads);
+        pdl_trigger();
+        const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::kFlagOff);
+        if (cta < plan.ctas) {
+            shared_prefix_role(plan, a.shared, maps.q, maps.k, maps.v, smem, smem_addr(smem + PrefixLayout::kPrefixBarOff), a.page_table,
+                               a.max_pages, a.num_pages, hkv, a.status, cta, tid, tmem);
+            return;
         }
-    } else {
-        pdl_wait();      // everything below reads what earlier kernels on the stream wrote
+        cta -= plan.ctas;
+        ctas -= plan.ctas;
+        if (warp == kPrefixTmemWarp) tmem_dealloc(tmem, kPrefixTmemCols);
+        __syncthreads();        // the tables of the partition have been read; the area is used again
     }
 
     // The lengths as they are now (one per thread: a launch takes at most kMaxBatchPerLaunch <= blockDim streams).
@@ -281,29 +314,13 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
 
     // Streams with nothing to attend get a zero row (mode 0) or an empty partial (mode 1); in mode 2 the empty
     // partial takes part in the exchange like any other (the other ranks wait for this rank's copy of every row).
-    volatile uint32_t* exchange_words = reinterpret_cast<volatile uint32_t*>(smem + SharedLayout::kExchangeOff);
+    volatile uint32_t* exchange_words = reinterpret_cast<volatile uint32_t*>(smem + L::kExchangeOff);
     ExchangeView xview = a.exchange;
     if (kExchange) {
-        xview = exchange_cache_peers(a.exchange, reinterpret_cast<unsigned char**>(smem + SharedLayout::kPeerOff), tid);
+        xview = exchange_cache_peers(a.exchange, reinterpret_cast<unsigned char**>(smem + L::kPeerOff), tid);
         __syncthreads();
     }
-    // Behind shared pages a stream without keys of its own still has the shared ones: those rows are written at the
-    // end, when the other launch's results are there.
-    auto write_streams_without_units = [&]() {
-        pdl_wait();
-        for (int s = blockIdx.x; s < a.batch; s += gridDim.x) {
-            if (prefix[s + 1] != prefix[s]) continue;
-            const int4 words = __ldcg(reinterpret_cast<const int4*>(a.shared.streams + s));
-            const SharedStream st{words.x, words.y, words.z, words.w};
-            for (int i = tid; i < 2 * hkv * kHeadDim; i += kConsumerThreads) {
-                float m = -CUDART_INF_F, l = 0.0f, o = 0.0f;
-                fold_shared(a.shared, st, i / (2 * kHeadDim), (i / kHeadDim) & 1, i % kHeadDim, m, l, o);
-                a.out[(size_t)s * (2 * hkv) * kHeadDim + i] = l > 0.0f ? (uint16_t)f32_to_bf16_bits(o / l) : (uint16_t)0;
-            }
-        }
-    };
-    if constexpr (!kShared)
-    for (int s = blockIdx.x; s < a.batch; s += gridDim.x) {
+    for (int s = cta; s < a.batch; s += ctas) {
         if (prefix[s + 1] != prefix[s]) continue;
         if (kExchange) {
             if (tid < kHeadDim) {        // warps 0-3, one row after the other
@@ -332,12 +349,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
     }
 
     const long long total_units = prefix[a.batch];
-    const long long grid_eff = total_units < (long long)gridDim.x ? total_units : (long long)gridDim.x;
-    const int cta = blockIdx.x;
-    if (cta >= grid_eff) {
-        if (kShared && warp < kConsumerWarps) write_streams_without_units();
-        return;
-    }
+    const long long grid_eff = total_units < (long long)ctas ? total_units : (long long)ctas;
+    if (cta >= grid_eff) return;
     const long long unit_begin = (long long)cta * total_units / grid_eff;
     const long long unit_end = (long long)(cta + 1) * total_units / grid_eff;
     const int count = (int)(unit_end - unit_begin);
@@ -382,7 +395,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
                     meta[2 * stage + 1] = make_int4(page_id, 0, 0, 0);
                     const size_t tile = ((size_t)page_id * hkv + head) * kTileElems;
                     const uint32_t dst = smem_addr(smem + stage * kStageBytes);
-                    const uint32_t staging = smem_addr(smem + SharedLayout::kQOff + stage * SharedLayout::kStagingBytes);
+                    const uint32_t staging = smem_addr(smem + L::kQOff + stage * L::kStagingBytes);
                     const bool new_segment = n == 0 || page_idx == 0;
                     constexpr uint32_t kQBytes = 2 * kHeadDim * 2;         // the two query heads of this KV head
                     constexpr uint32_t kRowBytes = kHeadDim * 2;
@@ -454,7 +467,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
                 const int head = seg % hkv;
                 const bool new_segment = n == 0 || page_idx == 0;
                 const bool last_page = page_idx == pages - 1;
-                unsigned char* staging = smem + SharedLayout::kQOff + stage * SharedLayout::kStagingBytes;
+                unsigned char* staging = smem + L::kQOff + stage * L::kStagingBytes;
                 if (new_segment || last_page) {
                     const uint2 craw = *reinterpret_cast<const uint2*>(staging + 512 + lane * 8);
                     const uint2 sraw = *reinterpret_cast<const uint2*>(staging + 768 + lane * 8);
@@ -499,7 +512,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
             atomicOr(a.status, QM_DEVSTAT_TIMEOUT);
         const int4 mt = meta[2 * stage];
         const int seg = mt.x, page_idx = mt.y, pages = mt.z, nvalid = mt.w;
-        unsigned char* staging = smem + SharedLayout::kQOff + stage * SharedLayout::kStagingBytes;
+        unsigned char* staging = smem + L::kQOff + stage * L::kStagingBytes;
         const int stream = seg / hkv;
         const int head = seg - stream * hkv;
 
@@ -652,13 +665,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
                 const float m = qh ? m1 : m0;
                 const bool whole = seg_from_start && page_idx == pages - 1;
                 const size_t row = (size_t)stream * (2 * hkv) + 2 * head + qh;
-                auto with_shared = [&](float m_own, float l_own, float o_own) {
-                    pdl_wait();
-                    const int4 words = __ldcg(reinterpret_cast<const int4*>(a.shared.streams + stream));
-                    const SharedStream st{words.x, words.y, words.z, words.w};
-                    fold_shared(a.shared, st, head, qh, d, m_own, l_own, o_own);
-                    return (uint16_t)f32_to_bf16_bits(o_own / l_own);
-                };
                 // `dead`: one of this thread's waits gave up (QM_DEVSTAT_TIMEOUT is set).  Its numbers are garbage
                 // and the unit description may be a stale one, so it writes nothing to global memory and takes
                 // no part in the arrival count; the barriers below are still passed by everyone.
@@ -668,8 +674,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
                         exchange_row(xview, (int)row, d, m * kLn2, lsum, sum, !dead, a.out + row * kHeadDim, a.status,
                                      exchange_words + 2 * qh, [qh] { if (qh) named_bar_sync(3, kHeadDim); else named_bar_sync(2, kHeadDim); });
                     } else if (dead) {
-                    } else if (kShared) {
-                        a.out[row * kHeadDim + d] = with_shared(m, lsum, sum);
                     } else if (a.mode == 0) {
                         a.out[row * kHeadDim + d] = (uint16_t)f32_to_bf16_bits(sum / lsum);
                     } else {
@@ -744,8 +748,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
                             exchange_row(xview, (int)row, d, big * kLn2, denom, acc, !dead, a.out + row * kHeadDim, a.status,
                                          exchange_words + 2 * qh, [qh] { if (qh) named_bar_sync(3, kHeadDim); else named_bar_sync(2, kHeadDim); });
                         } else if (dead) {
-                        } else if (kShared) {
-                            a.out[row * kHeadDim + d] = with_shared(big, denom, acc);
                         } else if (a.mode == 0) {
                             a.out[row * kHeadDim + d] = (uint16_t)f32_to_bf16_bits(acc / denom);
                         } else {
@@ -762,7 +764,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
             named_bar_sync(1, kConsumerThreads);
         }
     }
-    if (kShared) write_streams_without_units();
 }
 
 // ---------------------------------------------------------------------------
@@ -1116,15 +1117,15 @@ int32_t run_decode(qm_kv_pool* pool, int32_t layer, const uint16_t* q_rot, const
         if (mode == 2) {
             // the exchange is a variant of its own, so that the other modes compile without it
             QM_CUDA_TRY(qm_launch(qm_decode_splitkv_kernel<false, true>, dim3(grid), dim3(kDecodeThreads), SharedLayout::kTotal,
-                                  stream, a),
+                                  stream, a, NoMaps{}),
                         "split-KV decode attention with exchange launch");
         } else if (fused) {
             QM_CUDA_TRY(qm_launch(qm_decode_splitkv_kernel<true>, dim3(grid), dim3(kDecodeThreads), SharedLayout::kTotal,
-                                  stream, a),
+                                  stream, a, NoMaps{}),
                         "fused decode step launch");
         } else {
             QM_CUDA_TRY(qm_launch(qm_decode_splitkv_kernel<false>, dim3(grid), dim3(kDecodeThreads), SharedLayout::kTotal,
-                                  stream, a),
+                                  stream, a, NoMaps{}),
                         "split-KV decode attention launch");
         }
     }
@@ -1133,14 +1134,14 @@ int32_t run_decode(qm_kv_pool* pool, int32_t layer, const uint16_t* q_rot, const
 
 }  // namespace
 
-int32_t qm_launch_decode_behind_shared(qm_kv_pool* pool, int32_t layer, const uint16_t* q_rot, const int32_t* seq_lens,
-                                       const int32_t* page_table, int32_t max_pages, int32_t batch, uint16_t* out, void* workspace,
-                                       const SharedGroups& groups, cudaStream_t stream) {
+int32_t qm_launch_decode_shared(qm_kv_pool* pool, int32_t layer, const uint16_t* q_rot, const CUtensorMap& q_map, const int32_t* seq_lens,
+                                const int32_t* page_table, int32_t max_pages, int32_t batch, float* own_partials, void* workspace,
+                                const SharedGroups& groups, cudaStream_t stream) {
     static_assert(kSharedMaxBatch == kMaxBatchPerLaunch, "one launch");
+    auto kernel = qm_decode_splitkv_kernel<false, false, true, PrefixMaps>;
     static thread_local int attr_device = -1;
     if (attr_device != pool->device) {
-        QM_CUDA_TRY(cudaFuncSetAttribute(qm_decode_splitkv_kernel<false, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         SharedLayout::kTotalShared),
+        QM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PrefixLayout::kTotalShared),
                     "raise decode kernel shared memory");
         attr_device = pool->device;
     }
@@ -1153,7 +1154,7 @@ int32_t qm_launch_decode_behind_shared(qm_kv_pool* pool, int32_t layer, const ui
     a.value_pool = qm_kv_pool_value_ptr(pool, layer);
     a.seq_lens = seq_lens;
     a.page_table = page_table;
-    a.out = out;
+    a.partial_out = own_partials;
     a.ws_count = reinterpret_cast<int32_t*>(ws);
     a.ws_partials = reinterpret_cast<float*>(ws + kCounterRegionBytes);
     a.status = pool->status_dev;
@@ -1161,10 +1162,11 @@ int32_t qm_launch_decode_behind_shared(qm_kv_pool* pool, int32_t layer, const ui
     a.kv_heads = pool->kv_heads;
     a.max_pages = max_pages;
     a.num_pages = pool->num_pages;
+    a.mode = 1;
     a.shared = groups;
-    QM_CUDA_TRY(qm_launch(qm_decode_splitkv_kernel<false, false, true>, dim3(grid), dim3(kDecodeThreads), SharedLayout::kTotalShared,
-                          stream, a),
-                "split-KV decode attention behind shared pages launch");
+    const PrefixMaps maps{q_map, pool->key_maps[layer], pool->value_maps[layer]};
+    QM_CUDA_TRY(qm_launch(kernel, dim3(grid), dim3(kDecodeThreads), PrefixLayout::kTotalShared, stream, a, maps),
+                "decode attention over shared prefixes launch");
     return QM_OK;
 }
 

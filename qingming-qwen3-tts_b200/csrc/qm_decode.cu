@@ -281,7 +281,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
     if constexpr (kShared) {
         const SharedPlan plan = make_shared_plan(a.shared, a.seq_lens, a.batch, hkv, a.max_pages, (int)gridDim.x,
                                                  smem + L::kMergeOff, first_page, a.status, tid, kDecodeThreads);
-        pdl_trigger();
         const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::kFlagOff);
         if (cta < plan.ctas) {
             shared_prefix_role(plan, a.shared, maps.q, maps.k, maps.v, smem, smem_addr(smem + PrefixLayout::kPrefixBarOff), a.page_table,

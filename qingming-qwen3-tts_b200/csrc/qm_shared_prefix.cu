@@ -6,7 +6,7 @@
 // shared pages, each page once for up to 64 streams, on the tensor cores (qm_shared_prefix.cuh); the others the pages
 // behind them, stream by stream, as qm_decode_attention does.  The plan gives both kinds about the same number of pages
 // per CTA, so that they end together and HBM is busy to the end.  The second, below, folds a row's partial results: up to
-// a few dozen pieces of the shared part and one of its own, a CTA per row with all loads in flight at once.
+// a few dozen pieces of the shared part and one of its own, a CTA per pair of rows with its loads in flight together.
 #include "qm_shared_prefix.cuh"
 
 namespace {
@@ -27,71 +27,81 @@ __device__ __forceinline__ void fold_into(float& m, float& l, float4& o, float m
     m = top;
 }
 
-// Warp w folds the pieces w, w + 4, ... of the row, a lane four elements; then the four warps' results and the stream's
-// own part are folded in a fixed order.
-__global__ void __launch_bounds__(kCombineThreads) qm_shared_combine_kernel(const SharedGroups g, const float* own, int q_heads, uint16_t* out) {
-    __shared__ float4 part_o[kCombineWarps][32];
-    __shared__ float2 part_ml[kCombineWarps];
+// A CTA per (stream, KV head): the two query rows of the pair lie side by side in a piece's block.  Warp w folds the pieces
+// w, w + 4, ..., a lane four elements of both rows; then warp r folds row r's four results and the stream's own part, in
+// a fixed order.
+__global__ void __launch_bounds__(kCombineThreads) qm_shared_combine_kernel(const SharedGroups g, const float* own, int kv_heads, uint16_t* out) {
+    __shared__ float4 part_o[2][kCombineWarps][32];
+    __shared__ float2 part_ml[2][kCombineWarps];
     pdl_trigger();
     pdl_wait();
-    const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int stream = row / q_heads, head = row - stream * q_heads;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int stream = blockIdx.x / kv_heads, head = blockIdx.x - stream * kv_heads;
+    const size_t row0 = (size_t)blockIdx.x * 2;
     const int4 st = __ldcg(reinterpret_cast<const int4*>(g.streams + stream));     // base, splits, group_rows, row
-    const float* mine = own + (size_t)row * kOwnStride;
+    // the own part, fetched beside the descriptor
+    const float* mine = own + (row0 + (warp & 1)) * kOwnStride;
     const float2 own_ml = __ldcg(reinterpret_cast<const float2*>(mine));
-    const int first = st.x + (head >> 1) * st.y * st.z + st.w + (head & 1);
-    float m = -CUDART_INF_F, l = 0.0f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kFlight = 8;
+    const float2 own_a = __ldcg(reinterpret_cast<const float2*>(mine + 2 + 4 * lane));
+    const float2 own_b = __ldcg(reinterpret_cast<const float2*>(mine + 4 + 4 * lane));
+    const int first = st.x + head * st.y * st.z;
+    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.0f, 0.0f};
+    float4 o[2] = {};
+    constexpr int kFlight = 4;
     for (int j0 = warp; j0 < st.y; j0 += kFlight * kCombineWarps) {
-        float2 ml[kFlight];
-        float4 po[kFlight];
+        float2 ml[kFlight][2];
+        float4 po[kFlight][2];
 #pragma unroll
         for (int i = 0; i < kFlight; ++i) {
             const int j = j0 + i * kCombineWarps;
-            const size_t r = (size_t)(first + (j < st.y ? j : j0) * st.z);
-            ml[i] = __ldcg(g.partial_ml + r);
-            po[i] = __ldcg(reinterpret_cast<const float4*>(g.partial_o + r * kHeadDim + 4 * lane));
+            const size_t block = (size_t)(first + (j < st.y ? j : j0) * st.z);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                ml[i][r] = __ldcg(g.partial_ml + block + st.w + r);
+                po[i][r] = __ldcg(g.partial_o + block * (kHeadDim / 4) + (size_t)lane * st.z + st.w + r);
+            }
         }
 #pragma unroll
-        for (int i = 0; i < kFlight; ++i)
-            if (j0 + i * kCombineWarps < st.y) {
+        for (int i = 0; i < kFlight; ++i) {
+            if (j0 + i * kCombineWarps >= st.y) break;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
                 if (j0 == warp && i == 0) {
-                    m = ml[i].x;
-                    l = ml[i].y;
-                    o = po[i];
+                    m[r] = ml[i][r].x;
+                    l[r] = ml[i][r].y;
+                    o[r] = po[i][r];
                 } else {
-                    fold_into(m, l, o, ml[i].x, ml[i].y, po[i]);
+                    fold_into(m[r], l[r], o[r], ml[i][r].x, ml[i][r].y, po[i][r]);
                 }
             }
+        }
     }
-    part_o[warp][lane] = o;
-    if (lane == 0) part_ml[warp] = make_float2(m, l);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        part_o[r][warp][lane] = o[r];
+        if (lane == 0) part_ml[r][warp] = make_float2(m[r], l[r]);
+    }
     __syncthreads();
-    if (warp == 0) {
-        const float2 a = __ldcg(reinterpret_cast<const float2*>(mine + 2 + 4 * lane)), b = __ldcg(reinterpret_cast<const float2*>(mine + 4 + 4 * lane));
-        m = own_ml.x * kLog2e;
-        l = own_ml.y;
-        o = make_float4(a.x, a.y, b.x, b.y);
-        const bool any_own = l != 0.0f;           // a stream without keys of its own: m = -inf, l = 0, o = 0
-        bool first_part = !any_own;
+    if (warp < 2) {
+        float top = own_ml.x * kLog2e, sum = own_ml.y;
+        float4 acc = make_float4(own_a.x, own_a.y, own_b.x, own_b.y);
+        bool empty = sum == 0.0f;                 // a stream without keys of its own: m = -inf, l = 0, o = 0
 #pragma unroll
         for (int w = 0; w < kCombineWarps; ++w) {
             if (w >= st.y) break;
-            const float2 ml = part_ml[w];
-            if (first_part) {
-                m = ml.x;
-                l = ml.y;
-                o = part_o[w][lane];
-                first_part = false;
+            const float2 ml = part_ml[warp][w];
+            if (empty) {
+                top = ml.x;
+                sum = ml.y;
+                acc = part_o[warp][w][lane];
+                empty = false;
             } else {
-                fold_into(m, l, o, ml.x, ml.y, part_o[w][lane]);
+                fold_into(top, sum, acc, ml.x, ml.y, part_o[warp][w][lane]);
             }
         }
-        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-        uint2 bits = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-        uint16_t* dst = out + (size_t)row * kHeadDim + 4 * lane;
-        *reinterpret_cast<uint2*>(dst) = bits;
+        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+        *reinterpret_cast<uint2*>(out + (row0 + warp) * kHeadDim + 4 * lane) =
+            make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
     }
 }
 
@@ -169,7 +179,7 @@ int32_t qm_decode_attention_shared(qm_kv_pool* pool, int32_t layer, const uint16
     at += kDescriptorBytes;
     g.partial_ml = reinterpret_cast<float2*>(ws + at);
     at += align256(rows * sizeof(float2));
-    g.partial_o = reinterpret_cast<float*>(ws + at);
+    g.partial_o = reinterpret_cast<float4*>(ws + at);
     at += rows * kHeadDim * sizeof(float);
     float* own = reinterpret_cast<float*>(ws + at);
 
@@ -179,8 +189,8 @@ int32_t qm_decode_attention_shared(qm_kv_pool* pool, int32_t layer, const uint16
     rc = qm_launch_decode_shared(pool, layer, q_rot, q_map, seq_lens, page_table, max_pages, batch, own, workspace, g,
                                  static_cast<cudaStream_t>(stream));
     if (rc != QM_OK) return rc;
-    QM_CUDA_TRY(qm_launch(qm_shared_combine_kernel, dim3((unsigned)(batch * q_heads)), dim3(kCombineThreads), 0,
-                          static_cast<cudaStream_t>(stream), g, own, (int)q_heads, out),
+    QM_CUDA_TRY(qm_launch(qm_shared_combine_kernel, dim3((unsigned)(batch * pool->kv_heads)), dim3(kCombineThreads), 0,
+                          static_cast<cudaStream_t>(stream), g, own, (int)pool->kv_heads, out),
                 "shared-prefix combine launch");
     return QM_OK;
 }

@@ -30,7 +30,9 @@ struct SharedGroups {
     int groups;
     int max_pages;               // entries of `pages` are cut to this
     SharedStream* streams;       // workspace [kSharedMaxBatch]
-    float* partial_o;            // workspace [rows][128], unnormalised
+    // Workspace.  A piece's rows are a block of group_rows; in it the unnormalised outputs lie as [32][group_rows] float4
+    // (four elements of every row, then the next four), so that the threads that hold a row each store side by side.
+    float4* partial_o;
     float2* partial_ml;          // workspace [rows]: maximum (log2 domain) and sum of exponentials
 };
 
@@ -233,7 +235,7 @@ __device__ __forceinline__ void shared_prefix_tmem(uint32_t slot) {
     tc_fence_before();
 }
 
-// warps 0-3 softmax, warp 4 MMA issue, warp 5 TMA; the CTA's other warps only wait at its barriers.  `smem`: kPrefixTileBytes
+// warps 0-3 softmax, warp 4 MMA issue, warps 5 and 6 TMA; the CTA's other warps only wait at its barriers.  `smem`: kPrefixTileBytes
 // on a 1024-byte boundary.
 __device__ __forceinline__ void shared_prefix_role(const SharedPlan& plan, const SharedGroups& shared, const CUtensorMap& q_map,
                                                    const CUtensorMap& k_map, const CUtensorMap& v_map, unsigned char* smem, uint32_t bar0,
@@ -284,17 +286,23 @@ __device__ __forceinline__ void shared_prefix_role(const SharedPlan& plan, const
     };
     bool dead = false;
 
-    if (warp == 5) {
-        // ------------------------------------------------------------- TMA loads
+    if (warp == 5 || warp == 6) {
+        // --------------------------------------------- TMA loads: warp 5 queries and K, warp 6 V, neither behind the other
         if (lane == 0) {
+            const bool keys = warp == 5;
+            const int full = keys ? BAR_KFULL : BAR_VFULL, free = keys ? BAR_KFREE : BAR_VFREE;
+            const uint32_t ring = keys ? k_at : v_at;
+            const CUtensorMap* map = keys ? &k_map : &v_map;
             int n = 0, local = 0;
             for (int item = cta; item < plan.n_items; item += plan.ctas, ++local) {
                 const Item it = locate(item);
-                if (!mbar_wait_bounded(bar(BAR_QFREE), (local & 1) ^ 1, dead)) atomicOr(status, QM_DEVSTAT_TIMEOUT);
-                mbar_arrive_expect_tx(bar(BAR_Q), kPrefixQBytes);
-                for (int half = 0; half < 2; ++half)
-                    tma_load_3d(q_at + half * (kPrefixQBytes / 2), &q_map, bar(BAR_Q), half * 64, 2 * it.head,
-                                plan.starts[it.group] + it.tile * kStreamsPerTile);
+                if (keys) {
+                    if (!mbar_wait_bounded(bar(BAR_QFREE), (local & 1) ^ 1, dead)) atomicOr(status, QM_DEVSTAT_TIMEOUT);
+                    mbar_arrive_expect_tx(bar(BAR_Q), kPrefixQBytes);
+                    for (int half = 0; half < 2; ++half)
+                        tma_load_3d(q_at + half * (kPrefixQBytes / 2), &q_map, bar(BAR_Q), half * 64, 2 * it.head,
+                                    plan.starts[it.group] + it.tile * kStreamsPerTile);
+                }
                 const int32_t* table = page_table + (size_t)it.table_row * max_pages + it.page0;
                 int next_id = table[0];
                 for (int j = 0; j < it.pages; ++j, ++n) {
@@ -306,26 +314,17 @@ __device__ __forceinline__ void shared_prefix_role(const SharedPlan& plan, const
                     }
                     const int y = (id * hkv + it.head) * kPageTokens;
                     const int st = n % kPageStages;
-                    const uint32_t parity = ((n / kPageStages) & 1) ^ 1;
-                    if (!mbar_wait_bounded(bar(BAR_KFREE + st), parity, dead)) atomicOr(status, QM_DEVSTAT_TIMEOUT);
-                    mbar_arrive_expect_tx(bar(BAR_KFULL + st), kPageBytes);
+                    if (!mbar_wait_bounded(bar(free + st), ((n / kPageStages) & 1) ^ 1, dead)) atomicOr(status, QM_DEVSTAT_TIMEOUT);
+                    mbar_arrive_expect_tx(bar(full + st), kPageBytes);
                     for (int half = 0; half < 2; ++half)
-                        tma_load_2d(k_at + st * kPageBytes + half * (kPageBytes / 2), &k_map, bar(BAR_KFULL + st),
-                                    half * 64, y);
-                    if (!mbar_wait_bounded(bar(BAR_VFREE + st), parity, dead)) atomicOr(status, QM_DEVSTAT_TIMEOUT);
-                    mbar_arrive_expect_tx(bar(BAR_VFULL + st), kPageBytes);
-                    for (int half = 0; half < 2; ++half)
-                        tma_load_2d(v_at + st * kPageBytes + half * (kPageBytes / 2), &v_map, bar(BAR_VFULL + st),
-                                    half * 64, y);
+                        tma_load_2d(ring + st * kPageBytes + half * (kPageBytes / 2), map, bar(full + st), half * 64, y);
                 }
             }
             // every copy has landed (bounded) before this thread, and with it the CTA, goes
             bool gave_up = false;
-            if (local > 0) mbar_wait_bounded(bar(BAR_Q), (local - 1) & 1, gave_up);
-            for (int i = n > kPageStages ? n - kPageStages : 0; i < n; ++i) {
-                mbar_wait_bounded(bar(BAR_KFULL + i % kPageStages), (i / kPageStages) & 1, gave_up);
-                mbar_wait_bounded(bar(BAR_VFULL + i % kPageStages), (i / kPageStages) & 1, gave_up);
-            }
+            if (keys && local > 0) mbar_wait_bounded(bar(BAR_Q), (local - 1) & 1, gave_up);
+            for (int i = n > kPageStages ? n - kPageStages : 0; i < n; ++i)
+                mbar_wait_bounded(bar(full + i % kPageStages), (i / kPageStages) & 1, gave_up);
         }
         __syncwarp();
     } else if (warp == 4) {
@@ -450,7 +449,9 @@ __device__ __forceinline__ void shared_prefix_role(const SharedPlan& plan, const
             // ---- (m, l, o) of this piece
             wait(BAR_O + ((n - 1) & 1), ((n - 1) >> 1) & 1);
             tc_fence_after();
-            const size_t r = (size_t)plan.rows[it.group] + (size_t)(it.head * it.splits + it.split) * (2 * group_streams) + 2 * place + (tid & 1);
+            const int group_rows = 2 * group_streams, row = 2 * place + (tid & 1);
+            const size_t block = (size_t)plan.rows[it.group] + (size_t)(it.head * it.splits + it.split) * group_rows;
+            float4* dst = shared.partial_o + block * (kHeadDim / 4) + row;
 #pragma unroll
             for (int cch = 0; cch < 4; ++cch) {
                 uint32_t oreg[32];
@@ -459,11 +460,11 @@ __device__ __forceinline__ void shared_prefix_role(const SharedPlan& plan, const
                 if (real && !dead) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<uint4*>(shared.partial_o + r * kHeadDim + cch * 32 + i) =
-                            make_uint4(oreg[i], oreg[i + 1], oreg[i + 2], oreg[i + 3]);
+                        dst[(size_t)(cch * 8 + i / 4) * group_rows] = make_float4(__uint_as_float(oreg[i]), __uint_as_float(oreg[i + 1]),
+                                                                                 __uint_as_float(oreg[i + 2]), __uint_as_float(oreg[i + 3]));
                 }
             }
-            if (real && !dead) shared.partial_ml[r] = make_float2(m_used, l);
+            if (real && !dead) shared.partial_ml[block + row] = make_float2(m_used, l);
             tc_fence_before();
         }
     }

@@ -113,6 +113,7 @@ static_assert(SharedPlan::kBytes <= kConsumerWarps * 2 * kHeadDim * 4, "the part
 static_assert(kPrefixTileBytes == kStages * kStageBytes, "the prefix role's tiles are the ring");
 static_assert(PrefixLayout::kPrefixBarOff % 8 == 0 && PrefixLayout::kMergeOff % 16 == 0, "alignment");
 static_assert(PrefixLayout::kTotalShared <= SharedLayout::kTotal, "two CTAs per SM");
+static_assert(kMaxBatchPerLaunch + 1 <= kDecodeThreads, "one word of each array per thread");
 
 __device__ __forceinline__ int clamp_len(int len, int max_pages, uint32_t* status) {
     if (len < 0) len = 0;
@@ -275,15 +276,27 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
             }
         }
     }
-    pdl_wait();      // everything below reads what earlier kernels on the stream wrote
+    if (!kShared) pdl_wait();      // everything below reads what earlier kernels on the stream wrote
 
     int cta = blockIdx.x, ctas = gridDim.x;
     if constexpr (kShared) {
-        const SharedPlan plan = make_shared_plan(a.shared, a.seq_lens, a.batch, hkv, a.max_pages, (int)gridDim.x,
-                                                 smem + L::kMergeOff, first_page, a.status, tid, kDecodeThreads);
+        // The plan, too, is worked out ahead of the wait from what the arrays hold then, and kept if they still do after it.
+        const SharedGroups& g = a.shared;
+        auto word = [&](const int32_t* array, int n) { return tid < n ? __ldcg(array + tid) : 0; };
+        const int old_len = word(a.seq_lens, a.batch), old_start = word(g.starts, g.groups + 1), old_pages = word(g.pages, g.groups);
+        auto make_plan = [&]() {
+            return make_shared_plan(g, a.seq_lens, a.batch, hkv, a.max_pages, (int)gridDim.x, smem + L::kMergeOff, first_page, tid,
+                                    kDecodeThreads);
+        };
+        SharedPlan plan = make_plan();
+        pdl_wait();
+        if (__syncthreads_or(word(a.seq_lens, a.batch) != old_len || word(g.starts, g.groups + 1) != old_start ||
+                             word(g.pages, g.groups) != old_pages))
+            plan = make_plan();
+        if (blockIdx.x == 0) publish_shared_plan(plan, g, a.batch, a.status, tid);
         const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::kFlagOff);
         if (cta < plan.ctas) {
-            shared_prefix_role(plan, a.shared, maps.q, maps.k, maps.v, smem, smem_addr(smem + PrefixLayout::kPrefixBarOff), a.page_table,
+            shared_prefix_role(plan, g, maps.q, maps.k, maps.v, smem, smem_addr(smem + PrefixLayout::kPrefixBarOff), a.page_table,
                                a.max_pages, a.num_pages, hkv, a.status, cta, tid, tmem);
             return;
         }

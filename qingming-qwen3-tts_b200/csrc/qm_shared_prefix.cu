@@ -120,8 +120,7 @@ int32_t encode_pair_map(CUtensorMap* map, const void* base, int heads, uint64_t 
     return QM_OK;
 }
 
-// Partial rows of the shared part: a piece has at least 1 / (2 * SMs) of all shared pages (of tiles x heads), so by length
-// there are no more than 2 * SMs pieces of 128 rows; cutting each (tile, head) on its own adds one piece each at most.
+// Partial rows of the shared part: there are no more pieces than CTAs, of 128 rows each, or one piece per (tile, head).
 size_t partial_rows(int sm_count, int batch, int kv_heads) { return (size_t)(2 * sm_count) * 128 + (size_t)2 * batch * kv_heads; }
 
 constexpr size_t kDescriptorBytes = (size_t)kSharedMaxBatch * sizeof(SharedStream);

@@ -11,7 +11,8 @@
 #include "qm_tcgen05.cuh"
 
 constexpr int kSharedMaxBatch = 256;       // streams (and groups) per call
-constexpr float kSharedPageCost = 1.2f;    // time of a shared page against a stream's own page, both 32 KB
+constexpr float kSharedPageCost = 0.95f;   // time of a shared page, in that of a stream's own page (32 KB each)
+constexpr float kSharedPieceCost = 1.0f;   // what a piece costs besides its pages, in the same unit
 constexpr int kSharedMinPiece = 2;         // pages
 constexpr int kStreamsPerTile = 64;        // streams whose 128 query rows of a KV head make one M tile
 
@@ -45,7 +46,7 @@ struct SharedPlan {
     int* pages;          // [groups] shared pages, 0 where no stream takes part
     int* items;          // [groups + 1] first piece of each group
     int* rows;           // [groups + 1] first partial row of each group
-    int* words;          // ctas, piece, own units
+    int* words;          // ctas, piece, own units, 1 where the boundaries were out of order
     int ctas, piece, n_items, groups;
 
     static constexpr int kBytes = (3 * (kSharedMaxBatch + 4) + 3 * kSharedMaxBatch + 4) * 4;
@@ -62,13 +63,13 @@ __device__ __forceinline__ int warp_sum_scan(int v, int lane) {
 }
 
 // Group boundaries into shared memory, forced into order and into 0 .. batch whatever the array holds (so that every
-// stream is in one group at most); streams outside all groups share nothing.  One warp.
-__device__ __forceinline__ void load_group_starts(const SharedGroups& g, int batch, int* starts, uint32_t* status, int lane) {
+// stream is in one group at most); streams outside all groups share nothing.  One warp; returns whether it had to.
+__device__ __forceinline__ bool load_group_starts(const SharedGroups& g, int batch, int* starts, int lane) {
     int carry = 0;
     bool bad = false;
     for (int base = 0; base <= g.groups; base += 32) {
         const int i = base + lane;
-        int v = i <= g.groups ? g.starts[i] : 0;
+        int v = i <= g.groups ? __ldcg(g.starts + i) : 0;
         const int given = v;
         v = v < 0 ? 0 : (v > batch ? batch : v);
 #pragma unroll
@@ -83,7 +84,7 @@ __device__ __forceinline__ void load_group_starts(const SharedGroups& g, int bat
         }
         carry = __shfl_sync(0xffffffffu, v, 31);
     }
-    if (bad) atomicOr(status, QM_DEVSTAT_BAD_POS);
+    return __any_sync(0xffffffffu, bad);
 }
 
 // The group of a stream, or -1.
@@ -99,12 +100,12 @@ __device__ __forceinline__ int group_of_stream(const int* starts, int groups, in
 
 __device__ __forceinline__ int tiles_of(int streams) { return (streams + kStreamsPerTile - 1) / kStreamsPerTile; }
 
-// Every CTA works the whole plan out for itself, from the same arrays; CTA 0 also writes down where each stream's
-// partial results will lie.  first_page[s] = pages of stream s that are attended for it.  `area`: SharedPlan::kBytes of
-// shared memory.  All threads of the CTA.
+// Every CTA works the whole plan out for itself, from the same arrays (read past the L1: it may do so twice, before and
+// after the launch in front has written them).  first_page[s] = pages of stream s that are attended for it.  `area`:
+// SharedPlan::kBytes of shared memory.  All threads of the CTA; ends with a barrier.
 __device__ __forceinline__ SharedPlan make_shared_plan(const SharedGroups& g, const int32_t* seq_lens, int batch, int kv_heads,
                                                        int max_pages, int grid, unsigned char* area, uint16_t* first_page,
-                                                       uint32_t* status, int tid, int threads) {
+                                                       int tid, int threads) {
     SharedPlan p;
     p.starts = reinterpret_cast<int*>(area);
     p.items = p.starts + kSharedMaxBatch + 4;
@@ -117,18 +118,19 @@ __device__ __forceinline__ SharedPlan make_shared_plan(const SharedGroups& g, co
     const int lane = tid & 31, warp = tid >> 5;
     int len = 0;
     if (tid < batch) {
-        len = seq_lens[tid];
+        len = __ldcg(seq_lens + tid);
         const int cap = max_pages * kPageTokens;
         len = len < 0 ? 0 : (len > cap ? cap : len);
     }
-    if (warp == 0) load_group_starts(g, batch, p.starts, status, lane);
+    bool out_of_order = false;
+    if (warp == 0) out_of_order = load_group_starts(g, batch, p.starts, lane);
     for (int i = tid; i < g.groups; i += threads) {
         p.leader[i] = kSharedMaxBatch;
         p.pages[i] = 0;
-        const int given = g.pages[i];
+        const int given = __ldcg(g.pages + i);
         p.rows[i] = given < 0 ? 0 : (given > g.max_pages ? g.max_pages : given);
     }
-    if (tid < 4) p.words[tid] = 0;
+    if (tid < 4) p.words[tid] = tid == 3 && out_of_order ? 1 : 0;
     __syncthreads();
     int own = 0;
     if (tid < batch) {
@@ -147,29 +149,53 @@ __device__ __forceinline__ SharedPlan make_shared_plan(const SharedGroups& g, co
     if (lane == 0 && own) atomicAdd(&p.words[2], own);
     __syncthreads();
     if (warp == 0) {
-        auto count = [&](int piece, bool by_length) {        // pieces of at most `piece` pages, or pages x heads x tiles
-            int n = 0;
-            for (int i = lane; i < g.groups; i += 32)
-                n += tiles_of(p.starts[i + 1] - p.starts[i]) * kv_heads * (by_length ? p.pages[i] : (p.pages[i] + piece - 1) / piece);
-            return __reduce_add_sync(0xffffffffu, n);
-        };
-        const int total = count(1, true), own_units = p.words[2];
+        int most = 0;
+        for (int i = lane; i < g.groups; i += 32) most = max(most, p.starts[i + 1] > p.starts[i] ? p.pages[i] : 0);
+        most = __reduce_max_sync(0xffffffffu, most);
+        const int own_units = p.words[2];
         int ctas = 0, piece = 1;
-        if (total > 0) {
-            const float weighted = kSharedPageCost * (float)total;
-            ctas = (int)((float)grid * weighted / (weighted + (float)own_units) + 0.5f);
-            const int most = own_units > 0 ? grid - 1 : grid;
-            ctas = ctas < 1 ? 1 : (ctas > most ? most : ctas);
-            piece = (total + ctas - 1) / ctas;
-            piece = piece < kSharedMinPiece ? kSharedMinPiece : piece;
-            // A little longer until there is one piece per CTA at most (a CTA with two sets the time of all); where there
-            // are more tiles x heads than CTAs that cannot be, and pieces go round.
-            int n = count(piece, false);
-            for (int tries = 0; tries < 24 && n > ctas; ++tries) {
-                piece += piece / 16 + 1;
-                n = count(piece, false);
+        if (most > 0) {
+            // Three lengths per lane: the longest prefix in 1 .. 32 and in 41 .. 320 parts, and 2 .. 33 pages.  One piece per
+            // CTA; the call takes as long as the slower kind of CTA, a piece or an equal share of the own pages.
+            float best = CUDART_INF_F;
+            int best_piece = most, best_count = 0;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                const int parts = k == 0 ? lane + 1 : 9 * (lane + 1) + 32;
+                const int length = k == 2 ? lane + kSharedMinPiece : max((most + parts - 1) / parts, kSharedMinPiece);
+                int n = 0;
+                for (int i = 0; i < g.groups; ++i)
+                    n += tiles_of(p.starts[i + 1] - p.starts[i]) * kv_heads * ((p.pages[i] + length - 1) / length);
+                const int left = grid - n;
+                float time = (float)length * kSharedPageCost + kSharedPieceCost;
+                if (own_units > 0) time = fmaxf(time, left > 0 ? (float)own_units / (float)left : CUDART_INF_F);
+                if (left >= 0 && time < best) {
+                    best = time;
+                    best_piece = length;
+                    best_count = n;
+                }
             }
-            ctas = ctas < n ? ctas : n;
+            float overall = best;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) overall = fminf(overall, __shfl_xor_sync(0xffffffffu, overall, off));
+            if (overall < CUDART_INF_F) {
+                const int from = __ffs(__ballot_sync(0xffffffffu, best == overall)) - 1;
+                piece = __shfl_sync(0xffffffffu, best_piece, from);
+                ctas = __shfl_sync(0xffffffffu, best_count, from);
+            } else {
+                // more tiles x heads than CTAs: whole prefixes go round the CTAs that their share of the pages gives them
+                piece = most;
+                long long total = 0;
+                int n = 0;
+                for (int i = 0; i < g.groups; ++i) {
+                    const int lots = p.pages[i] > 0 ? tiles_of(p.starts[i + 1] - p.starts[i]) * kv_heads : 0;
+                    n += lots;
+                    total += (long long)lots * p.pages[i];
+                }
+                ctas = (int)((float)grid * (float)total / ((float)total + (float)own_units));
+                ctas = ctas < 1 ? 1 : (own_units > 0 && ctas > grid - 1 ? grid - 1 : ctas);
+                ctas = ctas < n ? ctas : n;
+            }
         }
         int item_carry = 0, row_carry = 0;
         for (int base = 0; base < g.groups; base += 32) {
@@ -195,15 +221,19 @@ __device__ __forceinline__ SharedPlan make_shared_plan(const SharedGroups& g, co
     p.ctas = p.words[0];
     p.piece = p.words[1];
     p.n_items = p.items[g.groups];
-    if (blockIdx.x == 0 && tid < batch) {
-        int4 w = make_int4(0, 0, 0, 0);
-        if (p.part[tid]) {
-            const int group = group_of_stream(p.starts, g.groups, tid), first = p.starts[group];
-            w = make_int4(p.rows[group], (p.pages[group] + p.piece - 1) / p.piece, 2 * (p.starts[group + 1] - first), 2 * (tid - first));
-        }
-        *reinterpret_cast<int4*>(g.streams + tid) = w;
-    }
     return p;
+}
+
+// Where each stream's partial results will lie, for the launch that folds them.  One CTA, once the plan is final.
+__device__ __forceinline__ void publish_shared_plan(const SharedPlan& p, const SharedGroups& g, int batch, uint32_t* status, int tid) {
+    if (tid == 0 && p.words[3]) atomicOr(status, QM_DEVSTAT_BAD_POS);
+    if (tid >= batch) return;
+    int4 w = make_int4(0, 0, 0, 0);
+    if (p.part[tid]) {
+        const int group = group_of_stream(p.starts, g.groups, tid), first = p.starts[group];
+        w = make_int4(p.rows[group], (p.pages[group] + p.piece - 1) / p.piece, 2 * (p.starts[group + 1] - first), 2 * (tid - first));
+    }
+    *reinterpret_cast<int4*>(g.streams + tid) = w;
 }
 
 // ---- the shared pages ----------------------------------------------------------------------------------------------

@@ -502,8 +502,8 @@ int32_t qm_final_head_sample(qm_kv_pool* pool, const uint16_t* logits, int32_t b
  *                    uniforms[row] times their sum (uniforms in [0, 1); anything below is 0, anything above picks the
  *                    last kept entry)
  * T <= 0 (or NaN) picks the first entry of the order.  NaN scores are never drawn; -inf is a weight of zero; a row
- * without any score above -inf gives token -1 and probability 0.  Weights are exact to about 1e-14 of the largest
- * and their sums do not depend on timing: the same inputs give the same tokens.
+ * without any score above -inf gives token -1 and probability 0.  Weights are exact to about 1e-13
+ * (and 2^-46 of the largest) and their sums do not depend on timing: the same inputs give the same tokens.
  *   logits: row r at element r * row_stride (0: one row, many draws), bf16, or fp32 with logits_are_fp32 != 0; vocab from
  *   1 to 262144, no alignment needed beyond the element's
  *   temperature, top_k, top_p, min_p [batch]: each may be NULL (1, off, off, off)

@@ -24,6 +24,8 @@
 // latency; rows are few, so as many CTAs as fit work on one wave of them.
 #include <math_constants.h>
 
+#include <cfloat>
+
 #include "qm_cluster.cuh"
 
 namespace {
@@ -36,6 +38,7 @@ constexpr int kList = 512;
 constexpr int kIndexBits = 18;
 constexpr int kMaxVocab = 1 << kIndexBits;
 constexpr int kMaxCluster = 8;
+constexpr int kCtasPerSm = 3;
 constexpr int kTable = 64;
 constexpr double kUnit = 35184372088832.0;      // 2^45: the whole number that stands for weight 1
 
@@ -75,7 +78,7 @@ struct Smem {
     uint32_t found;
     // the chosen bin
     u64 before_mass;
-    uint32_t before_count, bin, population;
+    uint32_t before_count, bin;
 };
 
 __device__ __forceinline__ void st_cluster_u64(uint32_t addr, u64 v) {
@@ -108,22 +111,16 @@ __device__ __forceinline__ float key_score(u64 key) {
 __device__ __forceinline__ int key_index(u64 key) { return kMaxVocab - 1 - (int)(key & (kMaxVocab - 1)); }
 
 // 2^45 exp((x - top) / T):  e = (x - top) / T = k ln2 / 64 + r with |r| <= 2^-7.5; 2^(k / 64) from a table, exp(r) by the first
-// five terms of its series (the sixth is below 1e-13).  A float becomes a double by moving its fields, which takes a
-// zero or a subnormal for a number below 2^-126; where T is so small that this could be seen, by conversion.
+// five terms of its series (the sixth is below 1e-13).  A float becomes a double by moving its fields, which is a third of
+// the time of a conversion and takes a zero or a subnormal for a number below 2^-126; where T is so small that this could
+// be seen, by conversion.  For NaN and infinities the result means nothing: callers compare with the cutoff.
 struct Weigher {
     const double* table;
     double top, inverse;         // 1 / T
-    float top_f;
     bool convert;
+    bool infinite;               // top is +inf: only the scores equal to it have a weight
 
-    __device__ __forceinline__ double operator()(float x) const {
-        double wide;
-        if (convert) {
-            wide = (double)x;
-        } else {
-            const uint32_t bits = __float_as_uint(x);
-            wide = __hiloint2double((int)((bits & 0x80000000u) | (((bits & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(bits << 29));
-        }
+    __device__ __forceinline__ double exponential(double wide) const {
         const double e = (wide - top) * inverse;
         constexpr double kMagic = 6755399441055744.0;             // 1.5 * 2^52: the low word of a sum holds its rounding
         const double shifted = fma(e, 92.332482616893656877, kMagic);      // 64 / ln2
@@ -135,8 +132,17 @@ struct Weigher {
         p = fma(p, r, 1.0);
         p *= table[k & (kTable - 1)];
         const double w = __hiloint2double(__double2hiint(p) + (k >> 6) * (1 << 20), __double2loint(p));
-        return x == top_f ? kUnit : (e > -31.9 ? w : 0.0);        // below -31.9: less than half of 2^-45; also NaN
+        return e > -31.9 ? w : 0.0;                               // below: less than half of 2^-45
     }
+    __device__ __forceinline__ double common(float x) const {
+        const uint32_t bits = __float_as_uint(x);
+        return exponential(__hiloint2double((int)((bits & 0x80000000u) | (((bits & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(bits << 29)));
+    }
+    __device__ __noinline__ double rare(float x) const {
+        if (infinite) return x == (float)top ? kUnit : 0.0;
+        return exponential((double)x);
+    }
+    __device__ __forceinline__ double operator()(float x) const { return convert || infinite ? rare(x) : common(x); }
 };
 
 // The nearest whole number of 0 .. 2^45.
@@ -156,7 +162,7 @@ __device__ __forceinline__ T warp_inclusive(T v, int lane) {
 }
 
 template <bool kFp32>
-__global__ void __launch_bounds__(kThreads, 4) qm_sample_filtered_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kernel(const SampleArgs a) {
     extern __shared__ __align__(16) unsigned char raw[];
     Smem& s = *reinterpret_cast<Smem*>(raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -179,20 +185,52 @@ __global__ void __launch_bounds__(kThreads, 4) qm_sample_filtered_kernel(const S
     for (int i = tid; i < kBins; i += kThreads) s.own.count[i] = s.own.low[i] = s.own.high[i] = 0u;
     pdl_wait();
 
-    const uint16_t* row16 = static_cast<const uint16_t*>(a.logits) + (kFp32 ? 0 : (size_t)row * a.row_stride + begin);
-    const float* row32 = static_cast<const float*>(a.logits) + (kFp32 ? (size_t)row * a.row_stride + begin : 0);
-    // -0 becomes +0 (equal scores), NaN becomes -inf (never drawn)
-    auto score_at = [&](int i) { return fmaxf((kFp32 ? row32[i] : bf16_bits_to_f32(row16[i])) + 0.0f, -CUDART_INF_F); };
-    // f(score, index in the slice) for every entry above -inf
+    // The slice in blocks of 256 scores, eight to a lane, on 16-byte boundaries: `lead` scores of the first block and some of
+    // the last belong to others and are filled with -inf.
+    constexpr int kBytes = kFp32 ? 4 : 2;
+    const unsigned char* base = static_cast<const unsigned char*>(a.logits) + ((size_t)row * a.row_stride + begin) * kBytes;
+    const int lead = (int)((reinterpret_cast<uintptr_t>(base) & 15u) / kBytes);
+    base -= lead * kBytes;
+    const int blocks = (lead + n + 255) / 256;
+    struct Eight {
+        uint4 a, b;              // bf16: a alone
+    };
+    auto load = [&](int block) {
+        Eight e;
+        const int v = block * 256 + lane * 8;
+        if (v >= lead && v + 8 <= lead + n) {
+            e.a = *reinterpret_cast<const uint4*>(base + (size_t)v * kBytes);
+            if (kFp32) e.b = *reinterpret_cast<const uint4*>(base + (size_t)v * kBytes + 16);
+        } else {
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool in = v + j >= lead && v + j < lead + n;
+                if (kFp32) w[j] = in ? *reinterpret_cast<const uint32_t*>(base + (size_t)(v + j) * 4) : 0xff800000u;
+                else w[j] = in ? *reinterpret_cast<const uint16_t*>(base + (size_t)(v + j) * 2) : 0xff80u;
+            }
+            if (kFp32) {
+                e.a = make_uint4(w[0], w[1], w[2], w[3]);
+                e.b = make_uint4(w[4], w[5], w[6], w[7]);
+            } else {
+                e.a = make_uint4(w[0] | (w[1] << 16), w[2] | (w[3] << 16), w[4] | (w[5] << 16), w[6] | (w[7] << 16));
+            }
+        }
+        return e;
+    };
+    auto score = [](const Eight& e, int j) {
+        const uint32_t* w = kFp32 && j >= 4 ? reinterpret_cast<const uint32_t*>(&e.b) : reinterpret_cast<const uint32_t*>(&e.a);
+        if (kFp32) return __uint_as_float(w[j & 3]);
+        return __uint_as_float((j & 1) ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+    };
+    // f(block, index of the lane's first score in the slice, the eight): a warp has every eighth block, one ahead in flight
     auto sweep = [&](auto f) {
-        constexpr int kFlight = 8;
-        for (int i0 = tid; i0 < n; i0 += kThreads * kFlight) {
-            float x[kFlight];
-#pragma unroll
-            for (int u = 0; u < kFlight; ++u) x[u] = i0 + u * kThreads < n ? score_at(i0 + u * kThreads) : -CUDART_INF_F;
-#pragma unroll
-            for (int u = 0; u < kFlight; ++u)
-                if (x[u] > -CUDART_INF_F) f(x[u], i0 + u * kThreads);
+        if (warp >= blocks) return;
+        Eight next = load(warp);
+        for (int block = warp; block < blocks; block += kWarps) {
+            const Eight e = next;
+            if (block + kWarps < blocks) next = load(block + kWarps);
+            f(block, block * 256 + lane * 8 - lead, e);
         }
     };
 
@@ -202,14 +240,18 @@ __global__ void __launch_bounds__(kThreads, 4) qm_sample_filtered_kernel(const S
     {
         float top = -CUDART_INF_F;
         int at = 0;
-        sweep([&](float x, int i) {
-            if (x > top) {                        // indices rise: the lower of equals stays
-                top = x;
-                at = i;
+        sweep([&](int, int i, const Eight& e) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = score(e, j);
+                if (x > top) {                    // never NaN; indices rise, so the lower of equals stays
+                    top = x;
+                    at = i + j;
+                }
+                lowest = fminf(lowest, x > -CUDART_INF_F ? x : CUDART_INF_F);
             }
-            lowest = fminf(lowest, x);
         });
-        if (top > -CUDART_INF_F) best = entry_key(top, begin + at);
+        if (top > -CUDART_INF_F) best = entry_key(top + 0.0f, begin + at);
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
@@ -249,15 +291,25 @@ __global__ void __launch_bounds__(kThreads, 4) qm_sample_filtered_kernel(const S
     }
 
     const float top = key_score(best);
-    const Weigher weight{s.table, (double)top, 1.0 / (double)temperature, top, temperature < 0x1p-60f};
+    const Weigher weight{s.table, (double)top, 1.0 / (double)temperature, temperature < 0x1p-60f, top == CUDART_INF_F};
     // entries below this have no weight (a float next to it is either 32 T below the top, or no other float lies between)
-    const float cutoff = top == CUDART_INF_F ? top : top - 32.5f * temperature;
+    const float cutoff = top == CUDART_INF_F ? top : fmaxf(top - 32.5f * temperature, -FLT_MAX);
     // Bins even in z between the largest score and the lowest one that can matter.  Each operation is monotone, so a larger
     // score never has a larger bin; NaN (equal infinities, 0 * inf) comes only where all entries in question are equal or
     // the last of all, and is the last bin.
     const float per_bin = (float)kBins / fminf(top - lowest, 32.0f * temperature);
     auto bin_of = [&](float x) {
         return (int)(__float_as_uint(fminf((top - x) * per_bin, (float)(kBins - 1)) + 8388608.0f) & (kBins - 1));
+    };
+    // Eight weights without a branch between them, so that their chains of dependent operations overlap.
+    auto weigh = [&](const Eight& e, u64 (&q)[8]) {
+        if (weight.convert || weight.infinite) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[j] = whole(weight.rare(score(e, j)));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[j] = whole(weight.common(score(e, j)));
+        }
     };
     float threshold = -CUDART_INF_F;              // what stays: scores above it, and at it the indices up to threshold_index
     int threshold_index = -1;
@@ -270,11 +322,12 @@ __global__ void __launch_bounds__(kThreads, 4) qm_sample_filtered_kernel(const S
         u64 prefix = 0ull, limit = (u64)k;
         uint32_t ahead_count = 0;
         u64 ahead_mass = 0;
+        int found = 0;
         constexpr int kShifts[6] = {40, 30, 20, 10, 0, 0};
         // entries of the chosen bin that agree with the digits so far
         auto matches = [&](float x, int i) {
-            if (x < cutoff || bin_of(x) != bin || !stays(x, i)) return false;
-            return shift >= 64 || (entry_key(x, begin + i) >> shift) == (prefix >> shift);
+            if (!(x >= cutoff) || bin_of(x) != bin || !stays(x, i)) return false;
+            return shift >= 64 || (entry_key(x + 0.0f, begin + i) >> shift) == (prefix >> shift);
         };
         for (int round = 0; round < 6; ++round) {
             if (round > 0 || !bins_are_clear) {
@@ -282,22 +335,38 @@ __global__ void __launch_bounds__(kThreads, 4) qm_sample_filtered_kernel(const S
                 __syncthreads();
             }
             const int next = round > 0 ? kShifts[round - 1] : 0;
-            sweep([&](float x, int i) {
-                int b;
-                if (round == 0) {
-                    if (x < cutoff || !stays(x, i)) return;
-                    b = bin_of(x);
-                } else {
-                    if (!matches(x, i)) return;
-                    b = kBins - 1 - (int)((entry_key(x, begin + i) >> next) & (u64)(kBins - 1));
+            sweep([&](int, int i0, const Eight& e) {
+                int b[8];                         // -1: not in the game
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float x = score(e, j);
+                    b[j] = bin_of(x);
+                    bool in = x >= cutoff && stays(x, i0 + j);
+                    if (round > 0) {
+                        in = in && matches(x, i0 + j);
+                        b[j] = kBins - 1 - (int)((entry_key(x + 0.0f, begin + i0 + j) >> next) & (u64)(kBins - 1));
+                    }
+                    b[j] = in ? b[j] : -1;
                 }
-                atomicAdd(&s.own.count[b], 1u);
-                if (by_mass) {
-                    const u64 q = whole(weight(x));
-                    const uint32_t lo = (uint32_t)q;
-                    const uint32_t old = atomicAdd(&s.own.low[b], lo);
-                    const uint32_t hi = (uint32_t)(q >> 32) + (old + lo < lo ? 1u : 0u);
-                    if (hi) atomicAdd(&s.own.high[b], hi);
+                if (!by_mass) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (b[j] >= 0) atomicAdd(&s.own.count[b[j]], 1u);
+                    return;
+                }
+                // the low words first, all of them, then what carries into the high words
+                u64 q[8];
+                uint32_t old[8];
+                weigh(e, q);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    q[j] = b[j] >= 0 ? q[j] : 0ull;
+                    old[j] = (uint32_t)q[j] ? atomicAdd(&s.own.low[b[j]], (uint32_t)q[j]) : 0u;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t hi = (uint32_t)(q[j] >> 32) + (old[j] + (uint32_t)q[j] < old[j] ? 1u : 0u);
+                    if (hi) atomicAdd(&s.own.high[b[j]], hi);
                 }
             });
             sync_all();
@@ -312,8 +381,9 @@ __global__ void __launch_bounds__(kThreads, 4) qm_sample_filtered_kernel(const S
                     for (int r = 0; r < kMaxCluster; ++r) {
                         c[r] = lo[r] = hi[r] = 0u;
                         if (r < cluster) {
-                            c[r] = ld_cluster_u32(remote(&s.own.count[b], r));
-                            if (by_mass) {
+                            if (!by_mass) {
+                                c[r] = ld_cluster_u32(remote(&s.own.count[b], r));
+                            } else {
                                 lo[r] = ld_cluster_u32(remote(&s.own.low[b], r));
                                 hi[r] = ld_cluster_u32(remote(&s.own.high[b], r));
                             }
@@ -327,8 +397,9 @@ __global__ void __launch_bounds__(kThreads, 4) qm_sample_filtered_kernel(const S
                         mass += ((u64)hi[r] << 32) + lo[r];
                     }
                     for (int r = 0; r < cluster; ++r) {
-                        st_cluster_u32(remote(&s.sum.count[b], r), count);
-                        if (by_mass) {
+                        if (!by_mass) {
+                            st_cluster_u32(remote(&s.sum.count[b], r), count);
+                        } else {
                             st_cluster_u32(remote(&s.sum.low[b], r), (uint32_t)mass);
                             st_cluster_u32(remote(&s.sum.high[b], r), (uint32_t)(mass >> 32));
                         }
@@ -342,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 4) qm_sample_filtered_kernel(const S
 #pragma unroll
             for (int j = 0; j < kBinsPerThread; ++j) {
                 const int b = tid * kBinsPerThread + j;
-                c[j] = bins->count[b];
+                c[j] = by_mass ? 0u : bins->count[b];
                 m[j] = by_mass ? ((u64)bins->high[b] << 32) + bins->low[b] : 0ull;
                 count += c[j];
                 mass += m[j];
@@ -373,13 +444,12 @@ __global__ void __launch_bounds__(kThreads, 4) qm_sample_filtered_kernel(const S
                 limit = wanted > 1.0 ? (u64)wanted : 1ull;
             }
             int mine = -1;
-            uint32_t my_count = 0, my_population = 0;
+            uint32_t my_count = 0;
             u64 my_mass = 0;
 #pragma unroll
             for (int j = 0; j < kBinsPerThread; ++j) {
-                if (c[j] && (by_mass ? mb : (u64)cb) < limit) {
+                if ((by_mass ? m[j] != 0ull && mb < limit : c[j] != 0u && (u64)cb < limit)) {
                     mine = tid * kBinsPerThread + j;
-                    my_population = c[j];
                     my_count = cb;
                     my_mass = mb;
                 }
@@ -390,7 +460,6 @@ __global__ void __launch_bounds__(kThreads, 4) qm_sample_filtered_kernel(const S
             __syncthreads();
             if (mine >= 0 && s.found == (uint32_t)mine + 1u) {
                 s.bin = (uint32_t)mine;
-                s.population = my_population;
                 s.before_count = my_count;
                 s.before_mass = my_mass;
             }
@@ -403,25 +472,28 @@ __global__ void __launch_bounds__(kThreads, 4) qm_sample_filtered_kernel(const S
                 prefix |= (u64)(kBins - 1 - (int)s.bin) << next;
                 shift = next;
             }
-            if (s.population <= kList) break;
-        }
-        // ---- the bin's entries, from all CTAs into all CTAs
-        sweep([&](float x, int i) {
-            if (!matches(x, i)) return;
-            const uint32_t at = atomicAdd(&s.list_count, 1u);
-            if (at < kList) s.list[at] = entry_key(x, begin + i);
-        });
-        sync_all();
-        int found = 0;
-        for (int r = 0; r < cluster; ++r) {
-            const int there = (int)(cluster > 1 ? ld_cluster_u32(remote(&s.list_count, r)) : s.list_count);
-            for (int i = tid; i < there && found + i < kList; i += kThreads) {
-                const u64 key = cluster > 1 ? ld_cluster_u64(remote(&s.list[i], r)) : s.list[i];
-                s.all[found + i] = make_ulonglong2(key, by_mass ? whole(weight(key_score(key))) : 1ull);
+            // the bin's entries, from all CTAs into all CTAs, if the list holds them
+            sweep([&](int, int i0, const Eight& e) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (!matches(score(e, j), i0 + j)) continue;
+                    const uint32_t at = atomicAdd(&s.list_count, 1u);
+                    if (at < kList) s.list[at] = entry_key(score(e, j) + 0.0f, begin + i0 + j);
+                }
+            });
+            sync_all();
+            found = 0;
+            for (int r = 0; r < cluster; ++r) {
+                const int there = (int)(cluster > 1 ? ld_cluster_u32(remote(&s.list_count, r)) : s.list_count);
+                for (int i = tid; i < there && found + i < kList; i += kThreads) {
+                    const u64 key = cluster > 1 ? ld_cluster_u64(remote(&s.list[i], r)) : s.list[i];
+                    s.all[found + i] = make_ulonglong2(key, by_mass ? whole(weight(key_score(key))) : 1ull);
+                }
+                found += there;
             }
-            found += there;
+            if (found <= kList) break;
+            sync_all();                           // the others' lists have been looked at
         }
-        found = found < kList ? found : kList;
         __syncthreads();
         // rank by counting: what the larger keys measure
         u64 last = ~0ull;
@@ -456,39 +528,53 @@ __global__ void __launch_bounds__(kThreads, 4) qm_sample_filtered_kernel(const S
     if (cut_k) search(false, k, 1.0f, true);
     if (p < 1.0f) search(true, 0, p, !cut_k);
 
-    // ---- the draw: kept weights in index order; a warp has a run of whole rows of 32 entries
+    // ---- the draw: kept weights in index order, summed by blocks (the bins' place is free again)
     const u64 least = min_p > 0.0f ? (u64)ceil((double)fminf(min_p, 2.0f) * kUnit) : 0ull;
-    auto kept = [&](float x, int i) -> double {
-        if (x < cutoff || !stays(x, i)) return 0.0;
-        const double w = weight(x);
-        return whole(w) < least && x != top ? 0.0 : w;
-    };
-    const int run = (n + kWarps * 32 - 1) / (kWarps * 32) * 32;
-    const int from = warp * run, to = from + run < n ? from + run : n;
-    u64 mine = 0ull;
-    {
-        constexpr int kFlight = 8;
-        for (int i0 = from + lane; i0 < to; i0 += 32 * kFlight) {
-            float x[kFlight];
+    const bool filtered = threshold > -CUDART_INF_F || least > 0ull;
+    auto keep = [&](const Eight& e, int i0, u64 (&q)[8]) {
+        if (filtered) {
+            bool any = false;
 #pragma unroll
-            for (int u = 0; u < kFlight; ++u) x[u] = i0 + u * 32 < to ? score_at(i0 + u * 32) : -CUDART_INF_F;
+            for (int j = 0; j < 8; ++j) any |= score(e, j) >= cutoff && stays(score(e, j), i0 + j);
+            if (!__any_sync(0xffffffffu, any)) {           // most blocks of a row that top-k or top-p has cut
 #pragma unroll
-            for (int u = 0; u < kFlight; ++u)
-                if (x[u] > -CUDART_INF_F) mine += whole(kept(x[u], i0 + u * 32));
+                for (int j = 0; j < 8; ++j) q[j] = 0ull;
+                return;
+            }
         }
-    }
+        weigh(e, q);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = score(e, j);
+            bool in = x >= cutoff;
+            if (filtered) in = in && stays(x, i0 + j) && (q[j] >= least || x == top);
+            q[j] = in ? q[j] : 0ull;
+        }
+    };
+    u64* block_sum = reinterpret_cast<u64*>(&s.own);
+    static_assert((kMaxVocab / 256 + 1) * sizeof(u64) <= sizeof(Bins), "block sums lie where the bins were");
+    __syncthreads();
+    u64 mine = 0ull;
+    sweep([&](int block, int i0, const Eight& e) {
+        u64 q[8], sum = 0ull;
+        keep(e, i0, q);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += q[j];
+        mine += sum;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (lane == 0) block_sum[block] = sum;
+    });
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);
     if (lane == 0) s.scan_mass[warp] = mine;
     __syncthreads();
-    u64 before = 0ull, total = 0ull;
+    u64 before = 0ull, own = 0ull;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += s.scan_mass[w];
-        total += s.scan_mass[w];
-    }
+    for (int w = 0; w < kWarps; ++w) own += s.scan_mass[w];
+    u64 total = own;
     if (cluster > 1) {
-        if (tid < cluster) st_cluster_u64(remote(&s.totals[rank], tid), total);
+        if (tid < cluster) st_cluster_u64(remote(&s.totals[rank], tid), own);
         cluster_sync_all();
         total = 0ull;
         for (int r = 0; r < cluster; ++r) {
@@ -499,33 +585,41 @@ __global__ void __launch_bounds__(kThreads, 4) qm_sample_filtered_kernel(const S
     const double wanted = (double)a.uniforms[row] * (double)total;
     u64 target = wanted > 0.0 ? (wanted < (double)total ? (u64)wanted : total - 1ull) : 0ull;
     if (target >= total) target = total - 1ull;
-    if (target < before || target >= before + mine) return;
-    // This warp's run holds it.  First which row of 32 entries: a lane adds up a row.  Then which entry: a lane has one.
+    if (warp > 0 || target < before || target >= before + own) return;
+    // The first warp of the CTA that has it: which block, which lane's eight, which of them.
     u64 sum = before;
-    for (int row0 = from; row0 < to; row0 += 32 * 32) {
-        u64 of_row = 0ull;
-        const int first = row0 + lane * 32;
-#pragma unroll 8
-        for (int i = 0; i < 32; ++i) {
-            const float x = first + i < to ? score_at(first + i) : -CUDART_INF_F;
-            if (x > -CUDART_INF_F) of_row += whole(kept(x, first + i));
-        }
-        const u64 up_to = sum + warp_inclusive(of_row, lane);
+    for (int block0 = 0; block0 < blocks; block0 += 32) {
+        const u64 q = block0 + lane < blocks ? block_sum[block0 + lane] : 0ull;
+        const u64 up_to = sum + warp_inclusive(q, lane);
         const unsigned past = __ballot_sync(0xffffffffu, target < up_to);
-        if (past) {
-            const int which = __ffs(past) - 1;
-            sum = __shfl_sync(0xffffffffu, up_to - of_row, which);
-            const int i = row0 + which * 32 + lane;
-            const float x = i < to ? score_at(i) : -CUDART_INF_F;
-            const double w = x > -CUDART_INF_F ? kept(x, i) : 0.0;
-            const unsigned beyond = __ballot_sync(0xffffffffu, target < sum + warp_inclusive(whole(w), lane));
-            if (lane == __ffs(beyond) - 1) {
-                a.tokens[row] = begin + i;
-                if (a.probs) a.probs[row] = (float)(w / (double)total);
-            }
-            return;
+        if (!past) {
+            sum = __shfl_sync(0xffffffffu, up_to, 31);
+            continue;
         }
-        sum = __shfl_sync(0xffffffffu, up_to, 31);
+        const int which = __ffs(past) - 1;
+        sum = __shfl_sync(0xffffffffu, up_to - q, which);
+        const int i0 = (block0 + which) * 256 + lane * 8 - lead;
+        const Eight e = load(block0 + which);
+        u64 kept[8], eight = 0ull;
+        keep(e, i0, kept);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) eight += kept[j];
+        const u64 to = sum + warp_inclusive(eight, lane);
+        const unsigned beyond = __ballot_sync(0xffffffffu, target < to);
+        if (lane == __ffs(beyond) - 1) {
+            u64 at = to - eight;
+            bool done = false;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                at += kept[j];
+                if (!done && target < at) {
+                    done = true;
+                    a.tokens[row] = begin + i0 + j;
+                    if (a.probs) a.probs[row] = (float)(weight(score(e, j)) / (double)total);
+                }
+            }
+        }
+        return;
     }
 }
 
@@ -543,8 +637,8 @@ extern "C" int32_t qm_sample_filtered(const void* logits, int32_t logits_are_fp3
                             reinterpret_cast<uintptr_t>(tokens_out) | reinterpret_cast<uintptr_t>(probs_out);
     if ((words & 3u) || (reinterpret_cast<uintptr_t>(logits) & (logits_are_fp32 ? 3u : 1u)))
         return qm_fail(QM_EINVAL, "misaligned tensor pointer");
-    // As many CTAs per row as leave each 2048 scores, up to eight, and no more than fit the GPU at a time (four per SM).
-    const long long fit = 4LL * sm_count_of_current_device();
+    // As many CTAs per row as leave each 2048 scores, up to eight, and no more than fit the GPU at a time.
+    const long long fit = (long long)kCtasPerSm * sm_count_of_current_device();
     int cluster = 1;
     while (cluster < kMaxCluster && vocab / (2 * cluster) >= 2048 && (long long)batch * 2 * cluster <= fit) cluster *= 2;
     if ((long long)batch * cluster > 0x7fffffffLL) return qm_fail(QM_ECAPACITY, "too many rows for one launch");

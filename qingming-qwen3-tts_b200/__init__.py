@@ -165,16 +165,15 @@ def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _packed(dtype, *tensors) -> None:
-    """The launchers take bare pointers: a tensor of another type or with gaps between its elements is refused here."""
-    for t in tensors:
-        if t is not None and (t.dtype != dtype or not t.is_cuda or not t.is_contiguous()):
-            raise ValueError(f"expected a contiguous CUDA tensor of {dtype}, got {t.dtype} on {t.device} with strides {t.stride()}")
-
-
-def _shaped(what: str, tensor, *shape) -> None:
-    if tensor is not None and tuple(tensor.shape) != shape:
-        raise ValueError(f"{what}: expected shape {shape}, got {tuple(tensor.shape)}")
+def _need(what: str, t, dtype, *shape) -> int:
+    """The address of a tensor for a launcher, which takes bare pointers: one of another type or shape, or with gaps
+    between its elements, is refused here.  None is a null pointer."""
+    if t is None:
+        return 0
+    if t.dtype is not dtype or t.shape != shape or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous CUDA tensor of {dtype} and shape {shape}, got {t.dtype}, {tuple(t.shape)} on "
+                         f"{t.device} with strides {t.stride()}")
+    return t.data_ptr()
 
 
 def _stream() -> int:
@@ -310,15 +309,9 @@ class TalkerAttention:
         group_starts[g + 1] - 1 share their first shared_pages[g] pages, which are read once for all of them."""
         import torch
 
-        batch, groups = q_rot.shape[0], shared_pages.shape[0]
+        bf16, i32 = torch.bfloat16, torch.int32
+        batch, groups, max_pages = q_rot.shape[0], shared_pages.shape[0], page_table.shape[1]
         out = torch.empty_like(q_rot) if out is None else out
-        _packed(torch.bfloat16, q_rot, out)
-        _packed(torch.int32, seq_lens, page_table, group_starts, shared_pages)
-        _shaped("q_rot", q_rot, batch, self.q_heads, HEAD_DIM)
-        _shaped("out", out, batch, self.q_heads, HEAD_DIM)
-        _shaped("seq_lens", seq_lens, batch)
-        _shaped("page_table", page_table, batch, page_table.shape[1])
-        _shaped("group_starts", group_starts, groups + 1)
         ws = self._shared_workspace
         if ws is None or self._shared_batch < batch:
             need = self.lib.qm_decode_shared_workspace_bytes(self.pool, batch)
@@ -326,8 +319,10 @@ class TalkerAttention:
             self._shared_batch = batch
             _check(self.lib.qm_decode_workspace_init(_ptr(ws), need, _stream()))
         _check(self.lib.qm_decode_attention_shared(
-            self.pool, layer, _ptr(q_rot), _ptr(seq_lens), _ptr(page_table), page_table.shape[1], batch, self.q_heads,
-            _ptr(group_starts), _ptr(shared_pages), groups, max_shared_pages, _ptr(out), _ptr(ws), ws.numel(), _stream()))
+            self.pool, layer, _need("q_rot", q_rot, bf16, batch, self.q_heads, HEAD_DIM), _need("seq_lens", seq_lens, i32, batch),
+            _need("page_table", page_table, i32, batch, max_pages), max_pages, batch, self.q_heads,
+            _need("group_starts", group_starts, i32, groups + 1), _need("shared_pages", shared_pages, i32, groups), groups,
+            max_shared_pages, _need("out", out, bf16, batch, self.q_heads, HEAD_DIM), ws.data_ptr(), ws.numel(), _stream()))
         return out
 
     def decode_step(self, layer, q, k, v, q_norm_weight, k_norm_weight, positions, page_table, out=None):
@@ -421,33 +416,23 @@ class TalkerAttention:
         rows, dim = x.shape
         q = x.new_empty((rows, dim), dtype=torch.int8) if q is None else q
         scale = x.new_empty((rows,), dtype=torch.float32) if scale is None else scale
-        _packed(torch.bfloat16, x, norm_weight)
-        _packed(torch.int8, q)
-        _packed(torch.float32, scale)
-        _shaped("norm_weight", norm_weight, dim)
-        _shaped("q", q, rows, dim)
-        _shaped("scale", scale, rows)
-        _check(self.lib.qm_quantize_rows_int8(_ptr(x), _ptr(norm_weight), self.epsilon, _ptr(q), _ptr(scale), rows, dim, _stream()))
+        _check(self.lib.qm_quantize_rows_int8(
+            _need("x", x, torch.bfloat16, rows, dim), _need("norm_weight", norm_weight, torch.bfloat16, dim), self.epsilon,
+            _need("q", q, torch.int8, rows, dim), _need("scale", scale, torch.float32, rows), rows, dim, _stream()))
         return q, scale
 
     def linear_int8(self, x, x_scale, weight, weight_scale, bias=None, residual=None, out=None):
         """bf16 rows from int8 rows and an int8 weight [out_features][in_features] with its scales."""
         import torch
 
+        i8, f32, bf16 = torch.int8, torch.float32, torch.bfloat16
         rows, inner = x.shape
         outer = weight.shape[0]
-        out = x.new_empty((rows, outer), dtype=torch.bfloat16) if out is None else out
-        _packed(torch.int8, x, weight)
-        _packed(torch.float32, x_scale, weight_scale)
-        _packed(torch.bfloat16, bias, residual, out)
-        _shaped("weight", weight, outer, inner)
-        _shaped("x_scale", x_scale, rows)
-        _shaped("weight_scale", weight_scale, outer)
-        _shaped("bias", bias, outer)
-        _shaped("residual", residual, rows, outer)
-        _shaped("out", out, rows, outer)
-        _check(self.lib.qm_linear_int8(self.pool, _ptr(x), _ptr(x_scale), _ptr(weight), _ptr(weight_scale), _ptr(bias),
-                                       _ptr(residual), _ptr(out), rows, outer, inner, _stream()))
+        out = x.new_empty((rows, outer), dtype=bf16) if out is None else out
+        _check(self.lib.qm_linear_int8(
+            self.pool, _need("x", x, i8, rows, inner), _need("x_scale", x_scale, f32, rows), _need("weight", weight, i8, outer, inner),
+            _need("weight_scale", weight_scale, f32, outer), _need("bias", bias, bf16, outer),
+            _need("residual", residual, bf16, rows, outer), _need("out", out, bf16, rows, outer), rows, outer, inner, _stream()))
         return out
 
     def qkv_linear_int8(self, x, x_scale, q_weight, q_scale, k_weight, k_scale, v_weight, v_scale, q_bias=None, k_bias=None,
@@ -455,43 +440,34 @@ class TalkerAttention:
         """The three projections of int8 rows; returns (q [rows][q_dim], k, v [rows][kv_dim]) in bf16."""
         import torch
 
+        i8, f32, bf16 = torch.int8, torch.float32, torch.bfloat16
         rows, inner = x.shape
+        q_dim, kv_dim = q_weight.shape[0], k_weight.shape[0]
         if out is None:
-            out = tuple(x.new_empty((rows, w.shape[0]), dtype=torch.bfloat16) for w in (q_weight, k_weight, v_weight))
-        _packed(torch.int8, x, q_weight, k_weight, v_weight)
-        _packed(torch.float32, x_scale, q_scale, k_scale, v_scale)
-        _packed(torch.bfloat16, q_bias, k_bias, v_bias, *out)
-        _shaped("x_scale", x_scale, rows)
-        for what, weight, scale, bias, o in (("q", q_weight, q_scale, q_bias, out[0]), ("k", k_weight, k_scale, k_bias, out[1]),
-                                             ("v", v_weight, v_scale, v_bias, out[2])):
-            outer = k_weight.shape[0] if what == "v" else weight.shape[0]
-            _shaped(what + " weight", weight, outer, inner)
-            _shaped(what + " scale", scale, outer)
-            _shaped(what + " bias", bias, outer)
-            _shaped(what + " output", o, rows, outer)
-        _check(self.lib.qm_qkv_linear_int8(
-            self.pool, _ptr(x), _ptr(x_scale), _ptr(q_weight), _ptr(q_scale), _ptr(q_bias), _ptr(k_weight), _ptr(k_scale),
-            _ptr(k_bias), _ptr(v_weight), _ptr(v_scale), _ptr(v_bias), _ptr(out[0]), _ptr(out[1]), _ptr(out[2]), rows, inner,
-            q_weight.shape[0], k_weight.shape[0], _stream()))
+            out = tuple(x.new_empty((rows, n), dtype=bf16) for n in (q_dim, kv_dim, kv_dim))
+        args = []
+        for what, weight, scale, bias, n in (("q", q_weight, q_scale, q_bias, q_dim), ("k", k_weight, k_scale, k_bias, kv_dim),
+                                             ("v", v_weight, v_scale, v_bias, kv_dim)):
+            args += [_need(what + "_weight", weight, i8, n, inner), _need(what + "_scale", scale, f32, n),
+                     _need(what + "_bias", bias, bf16, n)]
+        args += [_need("out", o, bf16, rows, n) for o, n in zip(out, (q_dim, kv_dim, kv_dim))]
+        _check(self.lib.qm_qkv_linear_int8(self.pool, _need("x", x, i8, rows, inner), _need("x_scale", x_scale, f32, rows), *args, rows,
+                                           inner, q_dim, kv_dim, _stream()))
         return out
 
     def gate_up_swiglu_int8(self, x, x_scale, gate_weight, gate_scale, up_weight, up_scale, out=None):
         """silu(gate) * up in bf16 from int8 rows and two int8 weights [intermediate][hidden]."""
         import torch
 
+        i8, f32 = torch.int8, torch.float32
         rows, inner = x.shape
         outer = gate_weight.shape[0]
         out = x.new_empty((rows, outer), dtype=torch.bfloat16) if out is None else out
-        _packed(torch.int8, x, gate_weight, up_weight)
-        _packed(torch.float32, x_scale, gate_scale, up_scale)
-        _packed(torch.bfloat16, out)
-        _shaped("x_scale", x_scale, rows)
-        for what, weight, scale in (("gate", gate_weight, gate_scale), ("up", up_weight, up_scale)):
-            _shaped(what + " weight", weight, outer, inner)
-            _shaped(what + " scale", scale, outer)
-        _shaped("out", out, rows, outer)
-        _check(self.lib.qm_gate_up_swiglu_int8(self.pool, _ptr(x), _ptr(x_scale), _ptr(gate_weight), _ptr(gate_scale),
-                                               _ptr(up_weight), _ptr(up_scale), _ptr(out), rows, inner, outer, _stream()))
+        _check(self.lib.qm_gate_up_swiglu_int8(
+            self.pool, _need("x", x, i8, rows, inner), _need("x_scale", x_scale, f32, rows),
+            _need("gate_weight", gate_weight, i8, outer, inner), _need("gate_scale", gate_scale, f32, outer),
+            _need("up_weight", up_weight, i8, outer, inner), _need("up_scale", up_scale, f32, outer),
+            _need("out", out, torch.bfloat16, rows, outer), rows, inner, outer, _stream()))
         return out
 
     def final_head_sample(self, logits, generation_index=None, history=None, flags=0, eos_token=2150,
@@ -521,17 +497,14 @@ class TalkerAttention:
         batch, vocab = logits.shape
         if logits.dtype not in (torch.bfloat16, torch.float32) or not logits.is_cuda or (vocab > 1 and logits.stride(1) != 1):
             raise ValueError("logits: expected CUDA rows of bfloat16 or float32 without gaps between their elements")
-        tokens = logits.new_empty((batch,), dtype=torch.int32) if tokens is None else tokens
-        probs = logits.new_empty((batch,), dtype=torch.float32) if probs is None else probs
-        _packed(torch.float32, uniforms, temperature, top_p, min_p, probs)
-        _packed(torch.int32, top_k, tokens)
-        for what, t in (("uniforms", uniforms), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p),
-                        ("tokens", tokens), ("probs", probs)):
-            _shaped(what, t, batch)
-        stride = logits.stride(0) if batch > 1 else vocab
-        _check(self.lib.qm_sample_filtered(_ptr(logits), int(logits.dtype == torch.float32), stride, batch, vocab, _ptr(uniforms),
-                                           _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(tokens), _ptr(probs),
-                                           _stream()))
+        f32, i32 = torch.float32, torch.int32
+        tokens = logits.new_empty((batch,), dtype=i32) if tokens is None else tokens
+        probs = logits.new_empty((batch,), dtype=f32) if probs is None else probs
+        _check(self.lib.qm_sample_filtered(
+            logits.data_ptr(), logits.dtype is f32, logits.stride(0) if batch > 1 else vocab, batch, vocab,
+            _need("uniforms", uniforms, f32, batch), _need("temperature", temperature, f32, batch), _need("top_k", top_k, i32, batch),
+            _need("top_p", top_p, f32, batch), _need("min_p", min_p, f32, batch), _need("tokens", tokens, i32, batch),
+            _need("probs", probs, f32, batch), _stream()))
         return tokens, probs
 
     def embedding_gather(self, table, token_ids, out=None):

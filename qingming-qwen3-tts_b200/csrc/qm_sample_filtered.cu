@@ -20,7 +20,7 @@
 // the CTAs add their bins up, a slice of them each, and every CTA finds the bin in which top-k (or top-p) ends by the
 // same scan.  The few entries of that bin are gathered and ranked by counting.  A bin with more than 512 entries
 // (many equal scores) is first cut down by digits of the entries' keys, which contain the index and therefore differ.
-// What bounds it: a weight takes eleven double-precision operations, and each step of the cluster a few microseconds of
+// What bounds it: a weight takes twelve double-precision operations, and each step of the cluster a few microseconds of
 // latency; rows are few, so as many CTAs as fit work on one wave of them.
 #include <math_constants.h>
 
@@ -39,7 +39,7 @@ constexpr int kIndexBits = 18;
 constexpr int kMaxVocab = 1 << kIndexBits;
 constexpr int kMaxCluster = 8;
 constexpr int kCtasPerSm = 3;
-constexpr int kTable = 64;
+constexpr int kTable = 16;                      // 128 bytes: lanes with different entries meet no bank twice
 constexpr double kUnit = 35184372088832.0;      // 2^45: the whole number that stands for weight 1
 
 typedef unsigned long long u64;
@@ -58,21 +58,22 @@ struct SampleArgs {
     int cluster;
 };
 
+// Behind the bins, a word per lane for the entries that are not in the game: adding them up there takes no branch.
 struct Bins {
-    uint32_t count[kBins];
-    uint32_t low[kBins];         // sums of the weights, low and high 32 bits
-    uint32_t high[kBins];
+    uint32_t count[kBins + 32];
+    uint32_t low[kBins + 32];    // sums of the weights, low and high 32 bits
+    uint32_t high[kBins + 32];
 };
 
 struct Smem {
     Bins own, sum;               // of this CTA; of the cluster
     u64 list[kList];             // this CTA's entries of the chosen bin
     ulonglong2 all[kList];       // the cluster's: key, weight
-    double table[kTable];        // 2^(j / 64) * 2^45
+    double table[kTable];        // 2^(j / 16) * 2^45
     u64 scan_mass[kWarps];
-    u64 best[kMaxCluster];       // one word from every CTA
+    float2 range[kMaxCluster];   // one from every CTA: largest and lowest score
     u64 totals[kMaxCluster];
-    float lowest[kMaxCluster];
+    float2 scan_range[kWarps];
     uint32_t scan_count[kWarps];
     uint32_t list_count;
     uint32_t found;
@@ -110,8 +111,8 @@ __device__ __forceinline__ float key_score(u64 key) {
 }
 __device__ __forceinline__ int key_index(u64 key) { return kMaxVocab - 1 - (int)(key & (kMaxVocab - 1)); }
 
-// 2^45 exp((x - top) / T):  e = (x - top) / T = k ln2 / 64 + r with |r| <= 2^-7.5; 2^(k / 64) from a table, exp(r) by the first
-// five terms of its series (the sixth is below 1e-13).  A float becomes a double by moving its fields, which is a third of
+// 2^45 exp((x - top) / T):  e = (x - top) / T = k ln2 / 16 + r with |r| <= ln2 / 32; 2^(k / 16) from a table, exp(r) by the first
+// six terms of its series (the seventh is below 2e-13).  A float becomes a double by moving its fields, which is a third of
 // the time of a conversion and takes a zero or a subnormal for a number below 2^-126; where T is so small that this could
 // be seen, by conversion.  For NaN and infinities the result means nothing: callers compare with the cutoff.
 struct Weigher {
@@ -123,15 +124,16 @@ struct Weigher {
     __device__ __forceinline__ double exponential(double wide) const {
         const double e = (wide - top) * inverse;
         constexpr double kMagic = 6755399441055744.0;             // 1.5 * 2^52: the low word of a sum holds its rounding
-        const double shifted = fma(e, 92.332482616893656877, kMagic);      // 64 / ln2
+        const double shifted = fma(e, 23.083120654223414219, kMagic);      // 16 / ln2
         const int k = __double2loint(shifted);
-        const double r = fma(shifted - kMagic, -0.010830424696249145, e);  // ln2 / 64
-        double p = fma(r, 1.0 / 24.0, 1.0 / 6.0);
+        const double r = fma(shifted - kMagic, -0.043321698784996581, e);  // ln2 / 16
+        double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+        p = fma(p, r, 1.0 / 6.0);
         p = fma(p, r, 0.5);
         p = fma(p, r, 1.0);
         p = fma(p, r, 1.0);
         p *= table[k & (kTable - 1)];
-        const double w = __hiloint2double(__double2hiint(p) + (k >> 6) * (1 << 20), __double2loint(p));
+        const double w = __hiloint2double(__double2hiint(p) + (k >> 4) * (1 << 20), __double2loint(p));
         return e > -31.9 ? w : 0.0;                               // below: less than half of 2^-45
     }
     __device__ __forceinline__ double common(float x) const {
@@ -234,63 +236,72 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
         }
     };
 
-    // ---- the first of the order, and the lowest score above -inf
-    u64 best = 0ull;
-    float lowest = CUDART_INF_F;
-    {
-        float top = -CUDART_INF_F;
-        int at = 0;
-        sweep([&](int, int i, const Eight& e) {
+    // ---- the largest score and the lowest above -inf, of the row
+    float top = -CUDART_INF_F, lowest = CUDART_INF_F;
+    sweep([&](int, int, const Eight& e) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = score(e, j);
-                if (x > top) {                    // never NaN; indices rise, so the lower of equals stays
-                    top = x;
-                    at = i + j;
-                }
-                lowest = fminf(lowest, x > -CUDART_INF_F ? x : CUDART_INF_F);
-            }
-        });
-        if (top > -CUDART_INF_F) best = entry_key(top + 0.0f, begin + at);
-    }
+        for (int j = 0; j < 8; ++j) {
+            const float x = score(e, j);
+            top = fmaxf(top, x);                  // never NaN
+            lowest = fminf(lowest, x > -CUDART_INF_F ? x : CUDART_INF_F);
+        }
+    });
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
-        const u64 other = __shfl_xor_sync(0xffffffffu, best, off);
-        best = other > best ? other : best;
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         lowest = fminf(lowest, __shfl_xor_sync(0xffffffffu, lowest, off));
     }
-    if (lane == 0) {
-        s.scan_mass[warp] = best;
-        s.scan_count[warp] = __float_as_uint(lowest);
-    }
+    if (lane == 0) s.scan_range[warp] = make_float2(top, lowest);
     __syncthreads();
     if (cluster > 1) cluster_wait();
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-        best = s.scan_mass[w] > best ? s.scan_mass[w] : best;
-        lowest = fminf(lowest, __uint_as_float(s.scan_count[w]));
+        top = fmaxf(top, s.scan_range[w].x);
+        lowest = fminf(lowest, s.scan_range[w].y);
     }
     if (cluster > 1) {
-        if (tid < cluster) {
-            st_cluster_u64(remote(&s.best[rank], tid), best);
-            st_cluster_u32(remote(&s.lowest[rank], tid), __float_as_uint(lowest));
-        }
+        if (tid < cluster)
+            st_cluster_u64(remote(&s.range[rank], tid), ((u64)__float_as_uint(lowest) << 32) | __float_as_uint(top));
         cluster_sync_all();
         for (int r = 0; r < cluster; ++r) {
-            best = s.best[r] > best ? s.best[r] : best;
-            lowest = fminf(lowest, s.lowest[r]);
+            top = fmaxf(top, s.range[r].x);
+            lowest = fminf(lowest, s.range[r].y);
         }
     }
+    top += 0.0f;                                  // -0 becomes +0
     const float temperature = a.temperature ? a.temperature[row] : 1.0f;
-    if (best == 0ull || !(temperature > 0.0f)) {  // nothing to draw from, or nothing to draw
+    if (top == -CUDART_INF_F || !(temperature > 0.0f)) {        // nothing to draw from, or nothing to draw
+        if (top == -CUDART_INF_F) {
+            if (rank == 0 && tid == 0) {
+                a.tokens[row] = -1;
+                if (a.probs) a.probs[row] = 0.0f;
+            }
+            return;
+        }
+        // the lowest index of the largest score
+        uint32_t at = 0xffffffffu;
+        sweep([&](int, int i0, const Eight& e) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (score(e, j) == top) at = min(at, (uint32_t)(begin + i0 + j));
+        });
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (lane == 0) s.scan_count[warp] = at;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) at = min(at, s.scan_count[w]);
+        if (cluster > 1) {
+            if (tid < cluster) st_cluster_u64(remote(&s.totals[rank], tid), at);
+            cluster_sync_all();
+            for (int r = 0; r < cluster; ++r) at = min(at, (uint32_t)s.totals[r]);
+        }
         if (rank == 0 && tid == 0) {
-            a.tokens[row] = best ? key_index(best) : -1;
-            if (a.probs) a.probs[row] = best ? 1.0f : 0.0f;
+            a.tokens[row] = (int)at;
+            if (a.probs) a.probs[row] = 1.0f;
         }
         return;
     }
 
-    const float top = key_score(best);
     const Weigher weight{s.table, (double)top, 1.0 / (double)temperature, temperature < 0x1p-60f, top == CUDART_INF_F};
     // entries below this have no weight (a float next to it is either 32 T below the top, or no other float lies between)
     const float cutoff = top == CUDART_INF_F ? top : fmaxf(top - 32.5f * temperature, -FLT_MAX);
@@ -312,8 +323,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
         }
     };
     float threshold = -CUDART_INF_F;              // what stays: scores above it, and at it the indices up to threshold_index
-    int threshold_index = -1;
-    auto stays = [&](float x, int i) { return x > threshold || (x == threshold && begin + i <= threshold_index); };
+    int threshold_index = -1;                     // (of the slice)
+    auto stays = [&](float x, int i) { return x > threshold || (x == threshold && i <= threshold_index); };
 
     // The last entry of the order, among those that stay so far, whose predecessors count less than k (by_mass false) or
     // weigh less than p times all of them: the new threshold.
@@ -336,22 +347,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
             }
             const int next = round > 0 ? kShifts[round - 1] : 0;
             sweep([&](int, int i0, const Eight& e) {
-                int b[8];                         // -1: not in the game
+                int b[8];
+                if (round == 0 && threshold == -CUDART_INF_F) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float x = score(e, j);
-                    b[j] = bin_of(x);
-                    bool in = x >= cutoff && stays(x, i0 + j);
-                    if (round > 0) {
-                        in = in && matches(x, i0 + j);
-                        b[j] = kBins - 1 - (int)((entry_key(x + 0.0f, begin + i0 + j) >> next) & (u64)(kBins - 1));
+                    for (int j = 0; j < 8; ++j) b[j] = score(e, j) >= cutoff ? bin_of(score(e, j)) : kBins + lane;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float x = score(e, j);
+                        const bool in = round > 0 ? matches(x, i0 + j) : x >= cutoff && stays(x, i0 + j);
+                        const int digit = kBins - 1 - (int)((entry_key(x + 0.0f, begin + i0 + j) >> next) & (u64)(kBins - 1));
+                        b[j] = in ? (round > 0 ? digit : bin_of(x)) : kBins + lane;
                     }
-                    b[j] = in ? b[j] : -1;
                 }
                 if (!by_mass) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (b[j] >= 0) atomicAdd(&s.own.count[b[j]], 1u);
+                    for (int j = 0; j < 8; ++j) atomicAdd(&s.own.count[b[j]], 1u);
                     return;
                 }
                 // the low words first, all of them, then what carries into the high words
@@ -359,10 +370,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
                 uint32_t old[8];
                 weigh(e, q);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    q[j] = b[j] >= 0 ? q[j] : 0ull;
-                    old[j] = (uint32_t)q[j] ? atomicAdd(&s.own.low[b[j]], (uint32_t)q[j]) : 0u;
-                }
+                for (int j = 0; j < 8; ++j) old[j] = atomicAdd(&s.own.low[b[j]], (uint32_t)q[j]);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const uint32_t hi = (uint32_t)(q[j] >> 32) + (old[j] + (uint32_t)q[j] < old[j] ? 1u : 0u);
@@ -518,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
         for (int w = 0; w < kWarps; ++w) last = s.scan_mass[w] < last ? s.scan_mass[w] : last;
         __syncthreads();
         threshold = key_score(last);
-        threshold_index = key_index(last);
+        threshold_index = key_index(last) - begin;
     };
 
     const int k = a.top_k ? a.top_k[row] : 0;
@@ -561,9 +569,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum += q[j];
         mine += sum;
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if (lane == 0) block_sum[block] = sum;
+        // the warp's sum in two steps of 24 bits (eight weights stay below 2^49): 32 lanes of either fit 32 bits
+        const u64 low = __reduce_add_sync(0xffffffffu, (uint32_t)sum & 0xffffffu), high = __reduce_add_sync(0xffffffffu, (uint32_t)(sum >> 24));
+        if (lane == 0) block_sum[block] = (high << 24) + low;
     });
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);

@@ -99,6 +99,36 @@ public:
               "Talker GQA2 M1 attention launch");
     }
 
+    // Decode append with the RoPE row and the cache slot of each new token given apart.
+    void launch_qk_norm_rope_cache_m1_sliced(int layer, const uint16_t* q, const uint16_t* k, const uint16_t* v,
+                                             const uint16_t* q_norm, const uint16_t* k_norm, const int32_t* positions,
+                                             const int32_t* cache_positions, const int32_t* page_table, int max_pages, int batch,
+                                             uint16_t* q_rotated) {
+        check(qm_decode_append_rope_sliced(pool_, layer, q, k, v, q_norm, k_norm, rope_cos_.as<uint16_t>(),
+                                           rope_sin_.as<uint16_t>(), rope_rows_, positions, cache_positions, page_table, max_pages,
+                                           batch, q_heads_, 1.0e-6f, q_rotated, stream_),
+              "Qingming QK norm/RoPE/cache launch (sliced)");
+    }
+
+    // Workspace of launch_attention_shared for up to `max_batch` streams (about 20 MB more than plain attention needs).
+    // Allocates: call it before serving, not while a stream is being captured.
+    void reserve_shared_prefixes(int max_batch) {
+        shared_workspace_ = DeviceBuffer(static_cast<std::size_t>(qm_decode_shared_workspace_bytes(pool_, max_batch)));
+        check(qm_decode_workspace_init(shared_workspace_.pointer, static_cast<int64_t>(shared_workspace_.bytes), stream_),
+              "Talker shared-prefix workspace");
+    }
+
+    // Decode attention for groups of streams whose page tables begin with the same pages (one voice prompt behind many
+    // requests): streams group_starts[g] .. group_starts[g + 1] - 1 share their first shared_pages[g] pages.
+    void launch_attention_shared(int layer, const uint16_t* query, const int32_t* seq_lens, const int32_t* page_table,
+                                 int max_pages, int batch, const int32_t* group_starts, const int32_t* shared_pages, int groups,
+                                 int max_shared_pages, uint16_t* context) {
+        check(qm_decode_attention_shared(pool_, layer, query, seq_lens, page_table, max_pages, batch, q_heads_, group_starts,
+                                         shared_pages, groups, max_shared_pages, context, shared_workspace_.pointer,
+                                         static_cast<int64_t>(shared_workspace_.bytes), stream_),
+              "Talker shared-prefix attention launch");
+    }
+
     // launch_qk_norm_rope_cache_m1 + launch_attention of one layer in a single launch (same bits).
     void decode_step(int layer, const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* q_norm,
                      const uint16_t* k_norm, const int32_t* positions, const int32_t* page_table, int max_pages,
@@ -170,6 +200,39 @@ public:
               "Qingming prefill gate/up/SwiGLU launch");
     }
 
+    // ---- the projections with 8-bit integer operands: rows and weights quantised by quantize_rows_int8 (norm_weight: RMSNorm
+    // in front, null for none), any number of rows
+    void quantize_rows_int8(const uint16_t* x, const uint16_t* norm_weight, int8_t* q, float* scale, int rows, int dim) {
+        check(qm_quantize_rows_int8(x, norm_weight, 1.0e-6f, q, scale, rows, dim, stream_), "row quantisation launch");
+    }
+    void linear_int8(const int8_t* x, const float* x_scale, const int8_t* weight, const float* weight_scale, const uint16_t* bias,
+                     const uint16_t* residual, uint16_t* output, int rows, int output_columns, int reduction_columns) {
+        check(qm_linear_int8(pool_, x, x_scale, weight, weight_scale, bias, residual, output, rows, output_columns,
+                             reduction_columns, stream_),
+              "8-bit linear launch");
+    }
+    void qkv_linear_int8(const int8_t* x, const float* x_scale, const int8_t* q_w, const float* q_s, const uint16_t* q_b,
+                         const int8_t* k_w, const float* k_s, const uint16_t* k_b, const int8_t* v_w, const float* v_s,
+                         const uint16_t* v_b, uint16_t* q, uint16_t* k, uint16_t* v, int rows, int hidden) {
+        check(qm_qkv_linear_int8(pool_, x, x_scale, q_w, q_s, q_b, k_w, k_s, k_b, v_w, v_s, v_b, q, k, v, rows, hidden,
+                                 q_heads_ * QM_HEAD_DIM, kv_heads_ * QM_HEAD_DIM, stream_),
+              "8-bit QKV launch");
+    }
+    void gate_up_swiglu_int8(const int8_t* x, const float* x_scale, const int8_t* gate_w, const float* gate_s, const int8_t* up_w,
+                             const float* up_s, uint16_t* output, int rows, int hidden, int intermediate) {
+        check(qm_gate_up_swiglu_int8(pool_, x, x_scale, gate_w, gate_s, up_w, up_s, output, rows, hidden, intermediate, stream_),
+              "8-bit gate/up/SwiGLU launch");
+    }
+
+    // Temperature, top-k, top-p, min-p and the draw from given uniform numbers, per row; each parameter array may be null.
+    void sample_filtered(const void* logits, bool logits_are_fp32, int64_t row_stride, int batch, int vocab, const float* uniforms,
+                         const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens,
+                         float* probs = nullptr) {
+        check(qm_sample_filtered(logits, logits_are_fp32 ? 1 : 0, row_stride, batch, vocab, uniforms, temperature, top_k, top_p,
+                                 min_p, tokens, probs, stream_),
+              "filtered sampling launch");
+    }
+
     // NativeFinalHead::run_fast_device after the head projection (17.cu:14475-14560) for every stream at once:
     // cast, repetition penalty, token suppression, greedy argmax (top_k = 0) or top-k sampling, history record.
     void final_head_sample(const uint16_t* logits, int batch, int vocab, int32_t* history, int history_capacity,
@@ -197,7 +260,7 @@ private:
     int q_heads_, kv_heads_, rope_rows_;
     cudaStream_t stream_;
     qm_kv_pool* pool_ = nullptr;
-    DeviceBuffer rope_cos_, rope_sin_, workspace_;
+    DeviceBuffer rope_cos_, rope_sin_, workspace_, shared_workspace_;
 };
 
 }  // namespace qm

@@ -165,14 +165,14 @@ def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _need(what: str, t, dtype, *shape) -> int:
-    """The address of a tensor for a launcher, which takes bare pointers: one of another type or shape, or with gaps
-    between its elements, is refused here.  None is a null pointer."""
+def _need(what: str, t, dtype, device: int, *shape) -> int:
+    """The address of a tensor for a launcher, which takes bare pointers: one of another type or shape, on another device
+    than the launch goes to, or with gaps between its elements, is refused here.  None is a null pointer."""
     if t is None:
         return 0
-    if t.dtype is not dtype or t.shape != shape or not t.is_cuda or not t.is_contiguous():
-        raise ValueError(f"{what}: expected a contiguous CUDA tensor of {dtype} and shape {shape}, got {t.dtype}, {tuple(t.shape)} on "
-                         f"{t.device} with strides {t.stride()}")
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous tensor of {dtype} and shape {shape} on cuda:{device}, got {t.dtype}, "
+                         f"{tuple(t.shape)} on {t.device} with strides {t.stride()}")
     return t.data_ptr()
 
 
@@ -309,6 +309,7 @@ class TalkerAttention:
         group_starts[g + 1] - 1 share their first shared_pages[g] pages, which are read once for all of them."""
         import torch
 
+        dev = torch.cuda.current_device()
         bf16, i32 = torch.bfloat16, torch.int32
         batch, groups, max_pages = q_rot.shape[0], shared_pages.shape[0], page_table.shape[1]
         out = torch.empty_like(q_rot) if out is None else out
@@ -319,10 +320,10 @@ class TalkerAttention:
             self._shared_batch = batch
             _check(self.lib.qm_decode_workspace_init(_ptr(ws), need, _stream()))
         _check(self.lib.qm_decode_attention_shared(
-            self.pool, layer, _need("q_rot", q_rot, bf16, batch, self.q_heads, HEAD_DIM), _need("seq_lens", seq_lens, i32, batch),
-            _need("page_table", page_table, i32, batch, max_pages), max_pages, batch, self.q_heads,
-            _need("group_starts", group_starts, i32, groups + 1), _need("shared_pages", shared_pages, i32, groups), groups,
-            max_shared_pages, _need("out", out, bf16, batch, self.q_heads, HEAD_DIM), ws.data_ptr(), ws.numel(), _stream()))
+            self.pool, layer, _need("q_rot", q_rot, bf16, dev, batch, self.q_heads, HEAD_DIM), _need("seq_lens", seq_lens, i32, dev, batch),
+            _need("page_table", page_table, i32, dev, batch, max_pages), max_pages, batch, self.q_heads,
+            _need("group_starts", group_starts, i32, dev, groups + 1), _need("shared_pages", shared_pages, i32, dev, groups), groups,
+            max_shared_pages, _need("out", out, bf16, dev, batch, self.q_heads, HEAD_DIM), ws.data_ptr(), ws.numel(), _stream()))
         return out
 
     def decode_step(self, layer, q, k, v, q_norm_weight, k_norm_weight, positions, page_table, out=None):
@@ -413,26 +414,28 @@ class TalkerAttention:
         for activations and, without a norm weight, for weight matrices."""
         import torch
 
+        dev = torch.cuda.current_device()
         rows, dim = x.shape
         q = x.new_empty((rows, dim), dtype=torch.int8) if q is None else q
         scale = x.new_empty((rows,), dtype=torch.float32) if scale is None else scale
         _check(self.lib.qm_quantize_rows_int8(
-            _need("x", x, torch.bfloat16, rows, dim), _need("norm_weight", norm_weight, torch.bfloat16, dim), self.epsilon,
-            _need("q", q, torch.int8, rows, dim), _need("scale", scale, torch.float32, rows), rows, dim, _stream()))
+            _need("x", x, torch.bfloat16, dev, rows, dim), _need("norm_weight", norm_weight, torch.bfloat16, dev, dim), self.epsilon,
+            _need("q", q, torch.int8, dev, rows, dim), _need("scale", scale, torch.float32, dev, rows), rows, dim, _stream()))
         return q, scale
 
     def linear_int8(self, x, x_scale, weight, weight_scale, bias=None, residual=None, out=None):
         """bf16 rows from int8 rows and an int8 weight [out_features][in_features] with its scales."""
         import torch
 
+        dev = torch.cuda.current_device()
         i8, f32, bf16 = torch.int8, torch.float32, torch.bfloat16
         rows, inner = x.shape
         outer = weight.shape[0]
         out = x.new_empty((rows, outer), dtype=bf16) if out is None else out
         _check(self.lib.qm_linear_int8(
-            self.pool, _need("x", x, i8, rows, inner), _need("x_scale", x_scale, f32, rows), _need("weight", weight, i8, outer, inner),
-            _need("weight_scale", weight_scale, f32, outer), _need("bias", bias, bf16, outer),
-            _need("residual", residual, bf16, rows, outer), _need("out", out, bf16, rows, outer), rows, outer, inner, _stream()))
+            self.pool, _need("x", x, i8, dev, rows, inner), _need("x_scale", x_scale, f32, dev, rows), _need("weight", weight, i8, dev, outer, inner),
+            _need("weight_scale", weight_scale, f32, dev, outer), _need("bias", bias, bf16, dev, outer),
+            _need("residual", residual, bf16, dev, rows, outer), _need("out", out, bf16, dev, rows, outer), rows, outer, inner, _stream()))
         return out
 
     def qkv_linear_int8(self, x, x_scale, q_weight, q_scale, k_weight, k_scale, v_weight, v_scale, q_bias=None, k_bias=None,
@@ -440,6 +443,7 @@ class TalkerAttention:
         """The three projections of int8 rows; returns (q [rows][q_dim], k, v [rows][kv_dim]) in bf16."""
         import torch
 
+        dev = torch.cuda.current_device()
         i8, f32, bf16 = torch.int8, torch.float32, torch.bfloat16
         rows, inner = x.shape
         q_dim, kv_dim = q_weight.shape[0], k_weight.shape[0]
@@ -448,10 +452,10 @@ class TalkerAttention:
         args = []
         for what, weight, scale, bias, n in (("q", q_weight, q_scale, q_bias, q_dim), ("k", k_weight, k_scale, k_bias, kv_dim),
                                              ("v", v_weight, v_scale, v_bias, kv_dim)):
-            args += [_need(what + "_weight", weight, i8, n, inner), _need(what + "_scale", scale, f32, n),
-                     _need(what + "_bias", bias, bf16, n)]
-        args += [_need("out", o, bf16, rows, n) for o, n in zip(out, (q_dim, kv_dim, kv_dim))]
-        _check(self.lib.qm_qkv_linear_int8(self.pool, _need("x", x, i8, rows, inner), _need("x_scale", x_scale, f32, rows), *args, rows,
+            args += [_need(what + "_weight", weight, i8, dev, n, inner), _need(what + "_scale", scale, f32, dev, n),
+                     _need(what + "_bias", bias, bf16, dev, n)]
+        args += [_need("out", o, bf16, dev, rows, n) for o, n in zip(out, (q_dim, kv_dim, kv_dim))]
+        _check(self.lib.qm_qkv_linear_int8(self.pool, _need("x", x, i8, dev, rows, inner), _need("x_scale", x_scale, f32, dev, rows), *args, rows,
                                            inner, q_dim, kv_dim, _stream()))
         return out
 
@@ -459,15 +463,16 @@ class TalkerAttention:
         """silu(gate) * up in bf16 from int8 rows and two int8 weights [intermediate][hidden]."""
         import torch
 
+        dev = torch.cuda.current_device()
         i8, f32 = torch.int8, torch.float32
         rows, inner = x.shape
         outer = gate_weight.shape[0]
         out = x.new_empty((rows, outer), dtype=torch.bfloat16) if out is None else out
         _check(self.lib.qm_gate_up_swiglu_int8(
-            self.pool, _need("x", x, i8, rows, inner), _need("x_scale", x_scale, f32, rows),
-            _need("gate_weight", gate_weight, i8, outer, inner), _need("gate_scale", gate_scale, f32, outer),
-            _need("up_weight", up_weight, i8, outer, inner), _need("up_scale", up_scale, f32, outer),
-            _need("out", out, torch.bfloat16, rows, outer), rows, inner, outer, _stream()))
+            self.pool, _need("x", x, i8, dev, rows, inner), _need("x_scale", x_scale, f32, dev, rows),
+            _need("gate_weight", gate_weight, i8, dev, outer, inner), _need("gate_scale", gate_scale, f32, dev, outer),
+            _need("up_weight", up_weight, i8, dev, outer, inner), _need("up_scale", up_scale, f32, dev, outer),
+            _need("out", out, torch.bfloat16, dev, rows, outer), rows, inner, outer, _stream()))
         return out
 
     def final_head_sample(self, logits, generation_index=None, history=None, flags=0, eos_token=2150,
@@ -494,17 +499,18 @@ class TalkerAttention:
         of the tokens among what the filters left)."""
         import torch
 
+        dev = torch.cuda.current_device()
         batch, vocab = logits.shape
-        if logits.dtype not in (torch.bfloat16, torch.float32) or not logits.is_cuda or (vocab > 1 and logits.stride(1) != 1):
-            raise ValueError("logits: expected CUDA rows of bfloat16 or float32 without gaps between their elements")
+        if logits.dtype not in (torch.bfloat16, torch.float32) or logits.get_device() != dev or (vocab > 1 and logits.stride(1) != 1):
+            raise ValueError(f"logits: expected rows of bfloat16 or float32 on cuda:{dev} without gaps between their elements")
         f32, i32 = torch.float32, torch.int32
         tokens = logits.new_empty((batch,), dtype=i32) if tokens is None else tokens
         probs = logits.new_empty((batch,), dtype=f32) if probs is None else probs
         _check(self.lib.qm_sample_filtered(
             logits.data_ptr(), logits.dtype is f32, logits.stride(0) if batch > 1 else vocab, batch, vocab,
-            _need("uniforms", uniforms, f32, batch), _need("temperature", temperature, f32, batch), _need("top_k", top_k, i32, batch),
-            _need("top_p", top_p, f32, batch), _need("min_p", min_p, f32, batch), _need("tokens", tokens, i32, batch),
-            _need("probs", probs, f32, batch), _stream()))
+            _need("uniforms", uniforms, f32, dev, batch), _need("temperature", temperature, f32, dev, batch), _need("top_k", top_k, i32, dev, batch),
+            _need("top_p", top_p, f32, dev, batch), _need("min_p", min_p, f32, dev, batch), _need("tokens", tokens, i32, dev, batch),
+            _need("probs", probs, f32, dev, batch), _stream()))
         return tokens, probs
 
     def embedding_gather(self, table, token_ids, out=None):

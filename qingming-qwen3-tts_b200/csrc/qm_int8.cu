@@ -272,7 +272,6 @@ qm_skinny_int8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_co
                       const __grid_constant__ CUtensorMap w3_map, const __grid_constant__ CUtensorMap x_map, const Int8Args a) {
     using L = SkinnySmem<kMPad>;
     constexpr int kTmemCols = kMPad < 32 ? 32 : kMPad;
-    pdl_trigger();
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw_addr = smem_addr(smem_raw);
     const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
@@ -320,6 +319,7 @@ qm_skinny_int8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_co
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+    pdl_trigger();           // not before this CTA has its TMEM: the next launch's CTAs hold theirs while they wait for this one
     bool dead = false;
     pdl_wait();
 
@@ -491,7 +491,6 @@ qm_rows_int8_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
                     const __grid_constant__ CUtensorMap w1_map, const __grid_constant__ CUtensorMap out_map, const Int8Args a) {
     using L = RowsSmem<kBN>;
     constexpr int kCols = kGated ? kBN / 2 : kBN;           // output columns per tile
-    pdl_trigger();
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw_addr = smem_addr(smem_raw);
     const uint32_t pad = (1024u - (raw_addr & 1023u)) & 1023u;
@@ -524,6 +523,7 @@ qm_rows_int8_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+    pdl_trigger();           // not before this CTA has its TMEM: the next launch's CTAs hold theirs while they wait for this one
     const int total_tiles = a.m_tiles * a.n_tiles;
     bool dead = false;
     pdl_wait();

@@ -151,6 +151,18 @@ def test_linear(eng, rows, inner, outer):
     assert torch.equal(eng.linear_int8(xq, xs, wq, ws, bias, residual), first), "the same call gives the same bits"
 
 
+@pytest.mark.parametrize("rows", [1, 40, 64, 65, 1000])
+@pytest.mark.parametrize("outer", [2048, 100, 37])
+def test_the_residual_may_be_the_output(eng, rows, outer):
+    import torch
+
+    xq, wq = levels(rows, rows, 512), levels(outer, outer, 512)
+    xs, ws, residual = scales(5, rows, 0.02), scales(6, outer, 0.01), numbers(8, rows, outer, scale=4.0)
+    want = eng.linear_int8(xq, xs, wq, ws, residual=residual)
+    assert eng.linear_int8(xq, xs, wq, ws, residual=residual, out=residual) is residual
+    assert torch.equal(residual, want)
+
+
 def test_the_largest_sums_are_exact(eng):
     import torch
 
@@ -272,6 +284,20 @@ def test_the_python_calls_check_their_tensors(eng):
                 lambda: eng.quantize_rows_int8(x, numbers(1, 63)), lambda: eng.linear_int8(xq, xs[:3], wq, ws),
                 lambda: eng.linear_int8(xq, xs, wq[:, :32], ws), lambda: eng.linear_int8(xq, xs, wq, ws[:5].contiguous()),
                 lambda: eng.linear_int8(xq, xs, wq, ws, bias=numbers(1, 31)),
-                lambda: eng.gate_up_swiglu_int8(xq, xs, wq, ws, wq[:16].contiguous(), ws)):
+                lambda: eng.gate_up_swiglu_int8(xq, xs, wq, ws, wq[:16].contiguous(), ws),
+                lambda: eng.linear_int8(xq.cpu(), xs, wq, ws), lambda: eng.quantize_rows_int8(x.cpu())):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_tensors_of_another_device_are_refused(eng, monkeypatch):
+    """The launch goes to the current device: here that is made to look like another one than the tensors'."""
+    import torch
+
+    x, (wq, ws) = numbers(1, 4, 64), (levels(2, 32, 64), scales(3, 32, 0.01))
+    xq, xs = eng.quantize_rows_int8(x)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for bad in (lambda: eng.quantize_rows_int8(x), lambda: eng.linear_int8(xq, xs, wq, ws), lambda: eng.gate_up_swiglu_int8(xq, xs, wq, ws, wq, ws),
+                lambda: eng.qkv_linear_int8(xq, xs, wq, ws, wq, ws, wq, ws), lambda: eng.sample_filtered(x.float(), xs)):
         with pytest.raises(ValueError):
             bad()

@@ -105,6 +105,8 @@ CASES = {
     "streams shorter than the prefix": dict(groups=[(6, 10), (2, 5)], own=[-1, 50, -64, -639, -640, 0]),
     "the first stream is idle": dict(groups=[(5, 20)], own=[None, 40, 1, 2, -30]),
     "streams outside the groups": dict(groups=[(4, 8), (3, 2)], own=[300, 20, 1], loose_front=3, loose_back=2),
+    "more tiles and heads than CTAs": dict(groups=[(2, i % 3 + 1) for i in range(40)], own=[9, 100, 0], kv_heads=16),
+    "pieces go round, nothing of their own": dict(groups=[(1, 1 + i % 4) for i in range(50)], own=[0], kv_heads=9),
     "every stream a group": dict(groups=[(1, i % 5) for i in range(40)], own=[9, 100, 0], kv_heads=2),
 }
 

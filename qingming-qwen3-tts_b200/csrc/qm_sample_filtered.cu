@@ -352,6 +352,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
 #pragma unroll
                     for (int j = 0; j < 8; ++j) b[j] = score(e, j) >= cutoff ? bin_of(score(e, j)) : kBins + lane;
                 } else {
+                    bool any = false;             // most blocks have nothing to add any more
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) any |= score(e, j) >= threshold && score(e, j) >= cutoff;
+                    if (!__any_sync(0xffffffffu, any)) return;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float x = score(e, j);
@@ -539,35 +543,49 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
     // ---- the draw: kept weights in index order, summed by blocks (the bins' place is free again)
     const u64 least = min_p > 0.0f ? (u64)ceil((double)fminf(min_p, 2.0f) * kUnit) : 0ull;
     const bool filtered = threshold > -CUDART_INF_F || least > 0ull;
-    auto keep = [&](const Eight& e, int i0, u64 (&q)[8]) {
-        if (filtered) {
-            bool any = false;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) any |= score(e, j) >= cutoff && stays(score(e, j), i0 + j);
-            if (!__any_sync(0xffffffffu, any)) {           // most blocks of a row that top-k or top-p has cut
-#pragma unroll
-                for (int j = 0; j < 8; ++j) q[j] = 0ull;
-                return;
-            }
-        }
-        weigh(e, q);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float x = score(e, j);
-            bool in = x >= cutoff;
-            if (filtered) in = in && stays(x, i0 + j) && (q[j] >= least || x == top);
-            q[j] = in ? q[j] : 0ull;
-        }
+    auto stays_in = [&](float x, int i) { return x >= cutoff && stays(x, i); };
+    auto kept = [&](float x, int i) -> u64 {
+        const u64 q = whole(weight(x));
+        return stays_in(x, i) && (q >= least || x == top) ? q : 0ull;
     };
     u64* block_sum = reinterpret_cast<u64*>(&s.own);
     static_assert((kMaxVocab / 256 + 1) * sizeof(u64) <= sizeof(Bins), "block sums lie where the bins were");
     __syncthreads();
     u64 mine = 0ull;
+    float* few = reinterpret_cast<float*>(&s.sum) + warp * 256;          // a warp's scores that stay, of one block
+    static_assert(kWarps * 256 * sizeof(float) <= sizeof(Bins), "they lie where the cluster's sums were");
     sweep([&](int block, int i0, const Eight& e) {
-        u64 q[8], sum = 0ull;
-        keep(e, i0, q);
+        u64 sum = 0ull;
+        if (!filtered) {
+            u64 q[8];
+            weigh(e, q);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum += q[j];
+            for (int j = 0; j < 8; ++j) sum += score(e, j) >= cutoff ? q[j] : 0ull;
+        } else {
+            // mostly few of the 256: side by side first, then a weight per lane
+            uint32_t mine = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mine |= score(e, j) >= threshold ? 1u << j : 0u;
+            if (!__any_sync(0xffffffffu, mine != 0u)) {
+                if (lane == 0) block_sum[block] = 0ull;
+                return;
+            }
+            mine = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mine |= stays_in(score(e, j), i0 + j) ? 1u << j : 0u;
+            const int upto = warp_inclusive(__popc(mine), lane), count = __shfl_sync(0xffffffffu, upto, 31);
+            int at = upto - __popc(mine);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (mine >> j & 1u) few[at++] = score(e, j);
+            __syncwarp();
+            for (int i = lane; i < count; i += 32) {
+                const float x = few[i];
+                const u64 q = whole(weight(x));
+                sum += q >= least || x == top ? q : 0ull;
+            }
+            __syncwarp();
+        }
         mine += sum;
         // the warp's sum in two steps of 24 bits (eight weights stay below 2^49): 32 lanes of either fit 32 bits
         const u64 low = __reduce_add_sync(0xffffffffu, (uint32_t)sum & 0xffffffu), high = __reduce_add_sync(0xffffffffu, (uint32_t)(sum >> 24));
@@ -608,10 +626,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
         sum = __shfl_sync(0xffffffffu, up_to - q, which);
         const int i0 = (block0 + which) * 256 + lane * 8 - lead;
         const Eight e = load(block0 + which);
-        u64 kept[8], eight = 0ull;
-        keep(e, i0, kept);
+        u64 q8[8], eight = 0ull;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) eight += kept[j];
+        for (int j = 0; j < 8; ++j) {
+            q8[j] = kept(score(e, j), i0 + j);
+            eight += q8[j];
+        }
         const u64 to = sum + warp_inclusive(eight, lane);
         const unsigned beyond = __ballot_sync(0xffffffffu, target < to);
         if (lane == __ffs(beyond) - 1) {
@@ -619,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
             bool done = false;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                at += kept[j];
+                at += q8[j];
                 if (!done && target < at) {
                     done = true;
                     a.tokens[row] = begin + i0 + j;

@@ -10,9 +10,10 @@
 // which is what a decode step streams, and the tensor pipe has twice the rate, which is what a prompt is bound by.
 //
 // Three kernels:
-//   qm_quantize_rows_kernel   one CTA per row; RMSNorm in front of the quantisation where a norm weight is given
+//   qm_quantize_rows_kernel   a CTA (many rows: a warp) per row; RMSNorm in front of the quantisation where a norm weight is given
 //   qm_skinny_int8_kernel     up to 64 token rows: the weight tile is the M operand, K split over a cluster
 //   qm_rows_int8_kernel       more rows: persistent 128-row tiles, two TMEM accumulators
+// (the figures below: one B200, launches in a row in a CUDA graph)
 #include <math_constants.h>
 
 #include "qm_cluster.cuh"
@@ -115,7 +116,8 @@ __device__ __forceinline__ uint2 quantize_eight(const uint4& raw, const uint4& w
     return packed;
 }
 
-// A CTA per row: few rows, each as fast as it goes; any width and alignment (kVector = false).
+// A CTA per row: few rows, each as fast as it goes; any width and alignment (kVector = false).  Bound by latency: 2.2 us for
+// one row of 2048, 3.4 us for 32 rows of 6144.
 template <bool kVector, bool kNorm>
 __global__ void __launch_bounds__(kQuantThreads) qm_quantize_rows_kernel(const uint16_t* __restrict__ x,
                                                                         const uint16_t* __restrict__ norm_weight,
@@ -175,12 +177,18 @@ __global__ void __launch_bounds__(kQuantThreads) qm_quantize_rows_kernel(const u
     }
 }
 
-// A warp per row: many rows.  Nothing but shuffles between the two sweeps, the second of which finds the row in L1.
+// A warp per row: many rows of up to 2048 values.  The row stays in registers (eight 16-byte pieces per lane, all
+// requested at once), and there is nothing but shuffles between its two sweeps.  14.9 us for 9923 rows of 2048 (4.1 TB/s of
+// the 9.4 us that HBM needs; 1.4 rounds of warps), 47.7 us for 40 099 (5.2 TB/s); with the norm 20.1 and 69.1 us, where a
+// lane reads the norm weight twice from the L1 and three CTAs per SM are faster than four (22.7, 73.0).
+constexpr int kManyRowsDim = 2048;
+
 template <bool kNorm>
-__global__ void __launch_bounds__(kQuantWarps * 32) qm_quantize_many_rows_kernel(const uint16_t* __restrict__ x,
+__global__ void __launch_bounds__(kQuantWarps * 32, kNorm ? 3 : 4) qm_quantize_many_rows_kernel(const uint16_t* __restrict__ x,
                                                                                 const uint16_t* __restrict__ norm_weight,
                                                                                 float epsilon, int8_t* __restrict__ q,
                                                                                 float* __restrict__ scale, int dim, int rows) {
+    constexpr int kPieces = kManyRowsDim / 8 / 32;
     pdl_wait();
     pdl_trigger();
     const int lane = threadIdx.x & 31;
@@ -190,21 +198,25 @@ __global__ void __launch_bounds__(kQuantWarps * 32) qm_quantize_many_rows_kernel
     const uint4* weights = reinterpret_cast<const uint4*>(norm_weight);
     const uint4 none = make_uint4(0u, 0u, 0u, 0u);
     const int vectors = dim / 8;
+    uint4 raw[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) raw[i] = lane + 32 * i < vectors ? src[lane + 32 * i] : none;
     RowSweep s = {0.0f, 0u};
-#pragma unroll 8
-    for (int v = lane; v < vectors; v += 32) sweep_eight<kNorm>(src[v], kNorm ? __ldg(weights + v) : none, s);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) sweep_eight<kNorm>(raw[i], kNorm && lane + 32 * i < vectors ? __ldg(weights + lane + 32 * i) : none, s);
     s.big_bits = __reduce_max_sync(0xffffffffu, s.big_bits);
 #pragma unroll
     for (int off = 16; off > 0 && kNorm; off >>= 1) s.sum += __shfl_xor_sync(0xffffffffu, s.sum, off);
     const QuantRow r = quant_row(s.big_bits);
     if (lane == 0) scale[row] = row_scale(r, s.sum, kNorm, dim, epsilon);
     uint2* dst = reinterpret_cast<uint2*>(q + (size_t)row * dim);
-#pragma unroll 4
-    for (int v = lane; v < vectors; v += 32) dst[v] = quantize_eight<kNorm>(src[v], kNorm ? __ldg(weights + v) : none, r);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+        if (lane + 32 * i < vectors)
+            dst[lane + 32 * i] = quantize_eight<kNorm>(raw[i], kNorm ? __ldg(weights + lane + 32 * i) : none, r);
 }
-// Measured with the norm, us, a CTA per row / a warp per row: 2048 columns, 2048 rows 6.5 / 7.5, 9923 rows 24.1 / 19.2;
-// 4096 columns, 16384 rows 71.6 / 74.9; 6144 columns, 9923 rows 60.3 / 76.4.
-constexpr int kManyRows = 4096, kManyRowsDim = 2048;
+// Measured, us, a CTA per row / a warp per row: 2048 columns, 2048 rows 6.5 / 7.5, 4096 rows 12.1 / 8.7, 9923 rows 24.1 / 14.9.
+constexpr int kManyRows = 4096;
 
 // ---- shared by the two products -----------------------------------------------------------------------------------
 
@@ -248,6 +260,9 @@ struct Int8Args {
 // range and fold their integer sums through distributed shared memory.  While the launch waits for its predecessor
 // (which writes the activations) it only asks the L2 for its weight slice: a weight matrix may be one that
 // the previous launch has just quantised, so no weight byte is read into the SM before the wait.
+//
+// Bound by latency (launch, copies after the wait, the cluster's fold): 4.0 us for one row of 2048 -> 2048 (4 MB of weights,
+// which HBM would bring in 0.64 us), 7.0 us for 32 rows of 6144 -> 2048, 9.1 us for 64 rows of 2048 -> 2 x 6144 gated.
 template <int kMPad>
 struct SkinnySmem {
     static constexpr int kStages = 4;
@@ -463,6 +478,11 @@ qm_skinny_int8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_co
 // its products are still running; results leave through a 2 KB block per warp and TMA stores, which also clip the
 // last tile.  kBN = 256 has the fewest operand bytes per operation; the narrower tiles are for calls whose 256-wide
 // tiles would leave SMs without one.
+//
+// Bound by operand bytes from the L2 (48 KB per 128 columns of K and SM; 670 cycles against 512 of the tensor pipe) and,
+// at small K, by the epilogue: 97 us = 2570 Tops for 9923 x 2048 x 6144, 187 us = 2940 Tops for 16384 x 4096 x 4096 (0.77
+// and 0.88 of twice the measured bf16 rate).  Four epilogue warps with scattered 16-byte stores and the column scales
+// read from global memory took 181 and 258 us.
 constexpr int kRowsThreads = 320;              // warps 0-7 epilogue, warp 8 MMA issue, warp 9 TMA loads
 constexpr int kRowsEpilogue = 256;
 constexpr int kStoreBytes = 32 * 32 * 2;       // 32 rows x 32 bf16 columns, 64-byte swizzle

@@ -5,8 +5,15 @@
 // Two launches.  The first (qm_decode_splitkv_kernel with kShared, qm_decode.cu) has CTAs of two kinds: some attend the
 // shared pages, each page once for up to 64 streams, on the tensor cores (qm_shared_prefix.cuh); the others the pages
 // behind them, stream by stream, as qm_decode_attention does.  The plan gives both kinds about the same number of pages
-// per CTA, so that they end together and HBM is busy to the end.  The second, below, folds a row's partial results: up to
+// per CTA, so that they end together and HBM is busy to the end (as two launches, the second one's CTAs came up
+// one by one where the first one's left, each with a full share still to do: 55 us against 43 for 64 streams behind 2048
+// tokens with up to 1024 of their own).  The second, below, folds a row's partial results: up to
 // a few dozen pieces of the shared part and one of its own, a CTA per pair of rows with its loads in flight together.
+//
+// Measured (8 KV heads): 64 streams behind 2048 tokens, up to 1024 of their own, 41-43 us (151 MB, 3.6 TB/s;
+// qm_decode_attention 100 us); 83 streams behind five prefixes of up to 4288 tokens, 48 us (184 us); 32 streams behind 32 768
+// tokens, 55 us (204 MB, 3.7 TB/s; 580 us).  What is left above the bytes' 22 to 31 us: about 3 us of plan, 4 us until the
+// first products, 6 us of fold, and CTAs with equal shares that end up to 10 us apart.
 #include "qm_shared_prefix.cuh"
 
 namespace {

@@ -11,8 +11,11 @@
 #include "qm_tcgen05.cuh"
 
 constexpr int kSharedMaxBatch = 256;       // streams (and groups) per call
-constexpr float kSharedPageCost = 0.95f;   // time of a shared page, in that of a stream's own page (32 KB each)
-constexpr float kSharedPieceCost = 1.0f;   // what a piece costs besides its pages, in the same unit
+// The costs that the cut goes by, in the time of a stream's own page.  Measured, us, at 0.85 / 0.95 / 1.05 per shared page: 64
+// streams behind 2048 tokens 42.8 / 43.0 / 44.2, 32 behind 32 768 tokens 53.2 / 54.4 / 56.2; at 3 instead of 1 per piece
+// 44.2 and 56.1.  Pieces of one page at least cost the first case 17.9 instead of 15.9 us of shared part alone.
+constexpr float kSharedPageCost = 0.95f;   // a shared page (32 KB like an own one)
+constexpr float kSharedPieceCost = 1.0f;   // a piece, besides its pages
 constexpr int kSharedMinPiece = 2;         // pages
 constexpr int kStreamsPerTile = 64;        // streams whose 128 query rows of a KV head make one M tile
 

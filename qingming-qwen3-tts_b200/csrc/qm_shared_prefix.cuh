@@ -16,6 +16,7 @@ constexpr int kSharedMaxBatch = 256;       // streams (and groups) per call
 // 44.2 and 56.1.  Pieces of one page at least cost the first case 17.9 instead of 15.9 us of shared part alone.
 constexpr float kSharedPageCost = 0.95f;   // a shared page (32 KB like an own one)
 constexpr float kSharedPieceCost = 1.0f;   // a piece, besides its pages
+constexpr int kOwnPartCost = 2;            // a stream's own part, besides its pages, per KV head (0 / 1 / 2: 83 streams behind five prefixes 50.7 / 48.0 / 47.5 us)
 constexpr int kSharedMinPiece = 2;         // pages
 constexpr int kStreamsPerTile = 64;        // streams whose 128 query rows of a KV head make one M tile
 
@@ -49,7 +50,7 @@ struct SharedPlan {
     int* pages;          // [groups] shared pages, 0 where no stream takes part
     int* items;          // [groups + 1] first piece of each group
     int* rows;           // [groups + 1] first partial row of each group
-    int* words;          // ctas, piece, own units, 1 where the boundaries were out of order
+    int* words;          // ctas, piece, cost of the own parts, 1 where the boundaries were out of order
     int ctas, piece, n_items, groups;
 
     static constexpr int kBytes = (3 * (kSharedMaxBatch + 4) + 3 * kSharedMaxBatch + 4) * 4;
@@ -146,7 +147,8 @@ __device__ __forceinline__ SharedPlan make_shared_plan(const SharedGroups& g, co
         }
         p.part[tid] = in;
         first_page[tid] = (uint16_t)(in ? shared : 0);
-        own = ((len + kPageTokens - 1) / kPageTokens - (in ? shared : 0)) * kv_heads;
+        own = (len + kPageTokens - 1) / kPageTokens - (in ? shared : 0);
+        own = own > 0 ? (own + kOwnPartCost) * kv_heads : 0;
     }
     own = __reduce_add_sync(0xffffffffu, own);
     if (lane == 0 && own) atomicAdd(&p.words[2], own);
@@ -155,7 +157,7 @@ __device__ __forceinline__ SharedPlan make_shared_plan(const SharedGroups& g, co
         int most = 0;
         for (int i = lane; i < g.groups; i += 32) most = max(most, p.starts[i + 1] > p.starts[i] ? p.pages[i] : 0);
         most = __reduce_max_sync(0xffffffffu, most);
-        const int own_units = p.words[2];
+        const int own_cost = p.words[2];
         int ctas = 0, piece = 1;
         if (most > 0) {
             // Three lengths per lane: the longest prefix in 1 .. 32 and in 41 .. 320 parts, and 2 .. 33 pages.  One piece per
@@ -171,7 +173,7 @@ __device__ __forceinline__ SharedPlan make_shared_plan(const SharedGroups& g, co
                     n += tiles_of(p.starts[i + 1] - p.starts[i]) * kv_heads * ((p.pages[i] + length - 1) / length);
                 const int left = grid - n;
                 float time = (float)length * kSharedPageCost + kSharedPieceCost;
-                if (own_units > 0) time = fmaxf(time, left > 0 ? (float)own_units / (float)left : CUDART_INF_F);
+                if (own_cost > 0) time = fmaxf(time, left > 0 ? (float)own_cost / (float)left : CUDART_INF_F);
                 if (left >= 0 && time < best) {
                     best = time;
                     best_piece = length;
@@ -195,8 +197,8 @@ __device__ __forceinline__ SharedPlan make_shared_plan(const SharedGroups& g, co
                     n += lots;
                     total += (long long)lots * p.pages[i];
                 }
-                ctas = (int)((float)grid * (float)total / ((float)total + (float)own_units));
-                ctas = ctas < 1 ? 1 : (own_units > 0 && ctas > grid - 1 ? grid - 1 : ctas);
+                ctas = (int)((float)grid * (float)total / ((float)total + (float)own_cost));
+                ctas = ctas < 1 ? 1 : (own_cost > 0 && ctas > grid - 1 ? grid - 1 : ctas);
                 ctas = ctas < n ? ctas : n;
             }
         }

@@ -441,7 +441,7 @@ int32_t qm_gate_up_swiglu_rows(qm_kv_pool* pool, const uint16_t* x, const uint16
  * fp32 scale per output channel, activations int8 with one fp32 scale per token row; the integer sums are exact:
  *   out[r][n] = bf16( float(sum_k x[r][k] * weight[n][k]) * x_scale[r] * weight_scale[n] + bias[n] + residual[r][n] )
  * with one rounding at the end.  qm_quantize_rows_int8 makes both operands (a weight matrix is a matrix of rows too).
- * Any number of rows: up to 64 go through a split-K cluster kernel, more through persistent 128-row tiles.
+ * Rows up to 2^31 - 256: up to 64 go through a split-K cluster kernel, more through persistent 128-row tiles.
  * in_features a multiple of 16, at most 65536; any out_features.  Tensors 16-byte aligned, x_scale 4-byte aligned;
  * bias and residual may be NULL.  The pool's device must be the current device. */
 
@@ -449,7 +449,8 @@ int32_t qm_gate_up_swiglu_rows(qm_kv_pool* pool, const uint16_t* x, const uint16
  * is x [rows][dim] bf16 itself or, with norm_weight [dim], RMSNorm(x) kept in fp32:
  * v[r][k] = x[r][k] * norm_weight[k] / sqrt(mean_k x[r][k]^2 + epsilon).  dim at most 24576, no alignment needed
  * beyond the element's (16-byte aligned x, norm_weight and 8-byte aligned q with dim a multiple of 8 are faster).
- * A row of zeros gets scale 0 and q 0; a row in which some x * norm_weight is not finite gets scale NaN and q 0, so that
+ * A row of zeros gets scale 0 and q 0 (so does the scale of a normalised row whose squares sum to infinity in fp32, as in
+ * every RMSNorm here); a row in which some x * norm_weight is not finite gets scale NaN and q 0, so that
  * everything computed from it is NaN. */
 int32_t qm_quantize_rows_int8(const uint16_t* x, const uint16_t* norm_weight, float epsilon, int8_t* q, float* scale,
                               int32_t rows, int32_t dim, void* stream);

@@ -26,6 +26,7 @@ namespace {
 constexpr int kQuantThreads = 256;             // CTA per row
 constexpr int kQuantWarps = 8;                 // warp per row
 constexpr int kQuantMaxDim = 24 * 1024;        // the row is staged in shared memory as bf16
+constexpr int kMaxRows = 0x7fffff00;           // a row number rounded up to the next tile is an int too
 
 // With a norm weight the value quantised is v[k] = x[k] * w[k] / rms; the rms divides out of q (q is a ratio of two such
 // values) and enters the scale alone, so one sweep collects both the sum of squares and the largest |x w|, and x w is
@@ -70,9 +71,10 @@ __device__ __forceinline__ QuantRow quant_row(uint32_t big_bits) {
 }
 
 __device__ __forceinline__ float row_scale(const QuantRow& r, float sum, bool norm, int dim, float epsilon) {
+    if (r.big == 0.0f) return 0.0f;               // also without an epsilon, where the root below is infinite
     float s = r.big / 127.0f;
     if (norm) s *= rsqrtf(sum / (float)dim + epsilon);
-    return r.flat && r.big != 0.0f ? CUDART_NAN_F : s;
+    return r.flat ? CUDART_NAN_F : s;
 }
 
 // The correctly rounded quotient 127 v / big (the product is exact: at most 7 + 16 bits), to the nearest whole number.
@@ -482,7 +484,9 @@ qm_skinny_int8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_co
 // Bound by operand bytes from the L2 (48 KB per 128 columns of K and SM; 670 cycles against 512 of the tensor pipe) and,
 // at small K, by the epilogue: 97 us = 2570 Tops for 9923 x 2048 x 6144, 187 us = 2940 Tops for 16384 x 4096 x 4096 (0.77
 // and 0.88 of twice the measured bf16 rate).  Four epilogue warps with scattered 16-byte stores and the column scales
-// read from global memory took 181 and 258 us.
+// read from global memory took 181 and 258 us.  Pairs of SMs on one tile of 256 x 256 (32 KB of operands instead of 48) gain
+// 1 to 3 % above 9000 rows, where the chip's power limit is near, and lose 6 % between 1500 and 4000 rows to their longer
+// start and end; walking the tiles in groups of 4 to 16 rows of tiles changes neither.
 constexpr int kRowsThreads = 320;              // warps 0-7 epilogue, warp 8 MMA issue, warp 9 TMA loads
 constexpr int kRowsEpilogue = 256;
 constexpr int kStoreBytes = 32 * 32 * 2;       // 32 rows x 32 bf16 columns, 64-byte swizzle
@@ -800,7 +804,7 @@ template <bool kGated>
 int32_t run_int8(qm_kv_pool* pool, const int8_t* x, const float* x_scale, const Int8Segment* segs, int n_segs, const int8_t* up,
                  const float* up_scale, const uint16_t* residual, int rows, int k_dim, cudaStream_t stream, const char* what) {
     if (!pool) return qm_fail(QM_EINVAL, "pool is null");
-    if (rows < 0) return qm_fail(QM_EINVAL, "rows must be >= 0");
+    if (rows < 0 || rows > kMaxRows) return qm_fail(QM_EINVAL, "rows must be >= 0 and at most 2^31 - 256");
     if (k_dim < 16 || k_dim % 16 != 0 || k_dim > 65536)
         return qm_fail(QM_EINVAL, "reduction width must be a positive multiple of 16, at most 65536");
     for (int i = 0; i < n_segs; ++i)
@@ -889,7 +893,8 @@ extern "C" {
 
 int32_t qm_quantize_rows_int8(const uint16_t* x, const uint16_t* norm_weight, float epsilon, int8_t* q, float* scale, int32_t rows,
                               int32_t dim, void* stream) {
-    if (rows < 0 || dim < 1 || dim > kQuantMaxDim) return qm_fail(QM_EINVAL, "dim must be between 1 and 24576");
+    if (rows < 0 || rows > kMaxRows) return qm_fail(QM_EINVAL, "rows must be >= 0 and at most 2^31 - 256");
+    if (dim < 1 || dim > kQuantMaxDim) return qm_fail(QM_EINVAL, "dim must be between 1 and 24576");
     if (rows == 0) return QM_OK;
     if (!x || !q || !scale) return qm_fail(QM_EINVAL, "null tensor pointer");
     const uintptr_t bf16s = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(norm_weight);

@@ -123,6 +123,18 @@ def test_rows_without_a_scale_and_at_the_ends_of_the_range(eng):
         assert np.array_equal(q[[4, 5, 7]].cpu().numpy(), np.rint(127 * wide / np.abs(wide).max(1, keepdims=True)))
 
 
+def test_a_row_of_zeros_without_an_epsilon(eng, monkeypatch):
+    """The root mean square is zero and its inverse infinite; the scale is 0 all the same."""
+    import torch
+
+    monkeypatch.setattr(eng, "epsilon", 0.0)
+    for rows, dim in ((3, 64), (3, 7), (5000, 64)):
+        x, w = numbers(1, rows, dim), numbers(2, dim) + 1
+        x[1] = 0
+        q, scale = eng.quantize_rows_int8(x, w)
+        assert scale[1] == 0 and not q[1].any() and torch.isfinite(scale).all() and bool((scale[2:] > 0).all())
+
+
 # ---- products
 
 def check_linear(got, xq, xs, wq, ws, bias=None, residual=None):
@@ -182,6 +194,43 @@ def test_many_tiles_of_every_width(eng, rows):
         xq, wq = levels(rows_here, rows_here, 256), levels(outer, outer, 256)
         xs, ws = scales(15, rows_here, 0.02), scales(16, outer, 0.01)
         check_linear(eng.linear_int8(xq, xs, wq, ws), xq, xs, wq, ws)
+
+
+@pytest.mark.parametrize("rows,inner,outer", [(2305, 16, 2049), (2432, 1040, 2041), (5000, 112, 1000), (18945, 144, 7), (130, 2048, 19200)])
+def test_the_widest_tiles_at_their_edges(eng, rows, inner, outer):
+    """Enough rows and columns for the widest tiles: last tiles of one row or one column, K of less than a chunk and of more
+    than the ring, several tiles to an SM."""
+    import torch
+
+    xq, wq = levels(rows, rows, inner), levels(outer, outer, inner)
+    xs, ws = scales(15, rows, 0.02), scales(16, outer, 0.01)
+    bias, residual = numbers(7, outer), numbers(8, rows, outer, scale=4.0)
+    whole, out = padded(rows, outer, torch.bfloat16)
+    check_linear(eng.linear_int8(xq, xs, wq, ws, out=out), xq, xs, wq, ws)
+    check_linear(eng.linear_int8(xq, xs, wq, ws, bias, residual, out=out), xq, xs, wq, ws, bias, residual)
+    assert bool((whole[rows:] == 7).all())
+    for _ in range(3):
+        assert torch.equal(eng.linear_int8(xq, xs, wq, ws, bias, residual), out)
+    other = slice(0, 70)                                   # the same rows in a small call
+    assert torch.equal(eng.linear_int8(xq[other], xs[other], wq, ws, bias, residual[other]), out[other])
+    if outer < 64:
+        return
+    of = 3.0 / (0.011 * 74 * 74 * inner ** 0.5)
+    gs, us, up = scales(4, outer, of), scales(5, outer, of), levels(3, outer, inner)
+    gated = eng.gate_up_swiglu_int8(xq, xs, wq, gs, up, us)
+    assert torch.equal(eng.gate_up_swiglu_int8(xq[other], xs[other], wq, gs, up, us), gated[other])
+    assert torch.equal(eng.gate_up_swiglu_int8(xq[-70:], xs[-70:], wq, gs, up, us), gated[-70:])
+
+
+def test_qkv_of_tiles_of_several_kinds(eng):
+    """Queries wide enough for the widest tiles, keys and values for narrow ones."""
+    import torch
+
+    xq, xs = levels(1, 2100, 272), scales(1, 2100, 0.02)
+    mats = [(levels(30 + i, n, 272), scales(40 + i, n, 0.01)) for i, n in enumerate((2304, 300, 300))]
+    got = eng.qkv_linear_int8(xq, xs, mats[0][0], mats[0][1], mats[1][0], mats[1][1], mats[2][0], mats[2][1])
+    for out, (w, s) in zip(got, mats):
+        check_linear(out, xq, xs, w, s)
 
 
 @pytest.mark.parametrize("rows", [1, 31, 64, 65, 300])

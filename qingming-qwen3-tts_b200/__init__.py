@@ -42,6 +42,7 @@ DEVSTAT_BAD_POS = 2
 DEVSTAT_TIMEOUT = 4
 
 HEAD_DIM = 128
+SHARED_MAX_BATCH = 256        # streams per launch_attention_shared
 PAGE_TOKENS = 64
 PARTIAL_STRIDE = HEAD_DIM + 2
 
@@ -306,7 +307,9 @@ class TalkerAttention:
 
     def launch_attention_shared(self, layer, q_rot, seq_lens, page_table, group_starts, shared_pages, max_shared_pages, out=None):
         """Decode attention for groups of streams whose tables begin with the same pages: streams group_starts[g] ..
-        group_starts[g + 1] - 1 share their first shared_pages[g] pages, which are read once for all of them."""
+        group_starts[g + 1] - 1 share their first shared_pages[g] pages, which are read once for all of them.  All calls of
+        one object use one workspace, made by the first of them (not while a stream is being captured) for the largest batch:
+        captured graphs keep it, and calls or replays must not overlap on the GPU."""
         import torch
 
         dev = torch.cuda.current_device()
@@ -314,10 +317,11 @@ class TalkerAttention:
         batch, groups, max_pages = q_rot.shape[0], shared_pages.shape[0], page_table.shape[1]
         out = torch.empty_like(q_rot) if out is None else out
         ws = self._shared_workspace
-        if ws is None or self._shared_batch < batch:
-            need = self.lib.qm_decode_shared_workspace_bytes(self.pool, batch)
+        if ws is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first launch_attention_shared makes its workspace and cannot be captured")
+            need = self.lib.qm_decode_shared_workspace_bytes(self.pool, SHARED_MAX_BATCH)
             self._shared_workspace = ws = torch.empty(need, dtype=torch.uint8, device="cuda")
-            self._shared_batch = batch
             _check(self.lib.qm_decode_workspace_init(_ptr(ws), need, _stream()))
         _check(self.lib.qm_decode_attention_shared(
             self.pool, layer, _need("q_rot", q_rot, bf16, dev, batch, self.q_heads, HEAD_DIM), _need("seq_lens", seq_lens, i32, dev, batch),

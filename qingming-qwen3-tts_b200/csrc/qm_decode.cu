@@ -283,16 +283,14 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
         // The plan, too, is worked out ahead of the wait from what the arrays hold then, and kept if they still do after it.
         const SharedGroups& g = a.shared;
         auto word = [&](const int32_t* array, int n) { return tid < n ? __ldcg(array + tid) : 0; };
-        const int old_len = word(a.seq_lens, a.batch), old_start = word(g.starts, g.groups + 1), old_pages = word(g.pages, g.groups);
-        auto make_plan = [&]() {
-            return make_shared_plan(g, a.seq_lens, a.batch, hkv, a.max_pages, (int)gridDim.x, smem + L::kMergeOff, first_page, tid,
-                                    kDecodeThreads);
+        auto make_plan = [&](int len, int start, int pages) {
+            return make_shared_plan(g, len, start, pages, a.batch, hkv, a.max_pages, (int)gridDim.x, smem + L::kMergeOff, first_page, tid);
         };
-        SharedPlan plan = make_plan();
+        const int old_len = word(a.seq_lens, a.batch), old_start = word(g.starts, g.groups + 1), old_pages = word(g.pages, g.groups);
+        SharedPlan plan = make_plan(old_len, old_start, old_pages);
         pdl_wait();
-        if (__syncthreads_or(word(a.seq_lens, a.batch) != old_len || word(g.starts, g.groups + 1) != old_start ||
-                             word(g.pages, g.groups) != old_pages))
-            plan = make_plan();
+        const int len = word(a.seq_lens, a.batch), start = word(g.starts, g.groups + 1), pages = word(g.pages, g.groups);
+        if (__syncthreads_or(len != old_len || start != old_start || pages != old_pages)) plan = make_plan(len, start, pages);
         if (blockIdx.x == 0) publish_shared_plan(plan, g, a.batch, a.status, tid);
         const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::kFlagOff);
         if (cta < plan.ctas) {

@@ -66,14 +66,14 @@ __device__ __forceinline__ int warp_sum_scan(int v, int lane) {
     return v;
 }
 
-// Group boundaries into shared memory, forced into order and into 0 .. batch whatever the array holds (so that every
-// stream is in one group at most); streams outside all groups share nothing.  One warp; returns whether it had to.
-__device__ __forceinline__ bool load_group_starts(const SharedGroups& g, int batch, int* starts, int lane) {
+// Group boundaries forced into order and into 0 .. batch whatever they are (so that every stream is in one group at
+// most); streams outside all groups share nothing.  One warp; returns whether it had to.
+__device__ __forceinline__ bool order_group_starts(int groups, int batch, int* starts, int lane) {
     int carry = 0;
     bool bad = false;
-    for (int base = 0; base <= g.groups; base += 32) {
+    for (int base = 0; base <= groups; base += 32) {
         const int i = base + lane;
-        int v = i <= g.groups ? __ldcg(g.starts + i) : 0;
+        int v = i <= groups ? starts[i] : 0;
         const int given = v;
         v = v < 0 ? 0 : (v > batch ? batch : v);
 #pragma unroll
@@ -82,7 +82,7 @@ __device__ __forceinline__ bool load_group_starts(const SharedGroups& g, int bat
             if (lane >= off) v = max(v, t);
         }
         v = max(v, carry);
-        if (i <= g.groups) {
+        if (i <= groups) {
             starts[i] = v;
             bad |= v != given;
         }
@@ -104,12 +104,12 @@ __device__ __forceinline__ int group_of_stream(const int* starts, int groups, in
 
 __device__ __forceinline__ int tiles_of(int streams) { return (streams + kStreamsPerTile - 1) / kStreamsPerTile; }
 
-// Every CTA works the whole plan out for itself, from the same arrays (read past the L1: it may do so twice, before and
-// after the launch in front has written them).  first_page[s] = pages of stream s that are attended for it.  `area`:
-// SharedPlan::kBytes of shared memory.  All threads of the CTA; ends with a barrier.
-__device__ __forceinline__ SharedPlan make_shared_plan(const SharedGroups& g, const int32_t* seq_lens, int batch, int kv_heads,
+// Every CTA works the whole plan out for itself, from word `tid` of each array in thread `tid` (it may do so twice, from what
+// it read before and after the launch in front has written them).  first_page[s] = pages of stream s that are attended for
+// it.  `area`: SharedPlan::kBytes of shared memory.  All threads of the CTA; ends with a barrier.
+__device__ __forceinline__ SharedPlan make_shared_plan(const SharedGroups& g, int len, int start, int shared_pages, int batch, int kv_heads,
                                                        int max_pages, int grid, unsigned char* area, uint16_t* first_page,
-                                                       int tid, int threads) {
+                                                       int tid) {
     SharedPlan p;
     p.starts = reinterpret_cast<int*>(area);
     p.items = p.starts + kSharedMaxBatch + 4;
@@ -120,20 +120,17 @@ __device__ __forceinline__ SharedPlan make_shared_plan(const SharedGroups& g, co
     p.words = p.pages + kSharedMaxBatch;
     p.groups = g.groups;
     const int lane = tid & 31, warp = tid >> 5;
-    int len = 0;
-    if (tid < batch) {
-        len = __ldcg(seq_lens + tid);
-        const int cap = max_pages * kPageTokens;
-        len = len < 0 ? 0 : (len > cap ? cap : len);
+    const int cap = max_pages * kPageTokens;
+    len = tid >= batch || len < 0 ? 0 : (len > cap ? cap : len);
+    if (tid <= g.groups) p.starts[tid] = start;
+    if (tid < g.groups) {
+        p.leader[tid] = kSharedMaxBatch;
+        p.pages[tid] = 0;
+        p.rows[tid] = shared_pages < 0 ? 0 : (shared_pages > g.max_pages ? g.max_pages : shared_pages);
     }
+    __syncthreads();
     bool out_of_order = false;
-    if (warp == 0) out_of_order = load_group_starts(g, batch, p.starts, lane);
-    for (int i = tid; i < g.groups; i += threads) {
-        p.leader[i] = kSharedMaxBatch;
-        p.pages[i] = 0;
-        const int given = __ldcg(g.pages + i);
-        p.rows[i] = given < 0 ? 0 : (given > g.max_pages ? g.max_pages : given);
-    }
+    if (warp == 0) out_of_order = order_group_starts(g.groups, batch, p.starts, lane);
     if (tid < 4) p.words[tid] = tid == 3 && out_of_order ? 1 : 0;
     __syncthreads();
     int own = 0;

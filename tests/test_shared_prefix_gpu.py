@@ -262,6 +262,33 @@ def test_captured_and_on_another_stream(qm):
     c.done()
 
 
+def test_a_captured_graph_keeps_its_workspace(qm, monkeypatch):
+    """A larger batch between the capture of a graph and its replay, and a smaller one after it."""
+    import torch
+
+    c = Case(qm, [(12, 11), (60, 3)], [33, 500, 0, 90], seed=21)
+    few = dict(q_rot=c.q[:5], seq_lens=c.seq[:5], page_table=c.table[:5], group_starts=torch.tensor([0, 5], dtype=torch.int32, device="cuda"),
+               shared_pages=c.pages[:1])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError):
+        c.run(**few)
+    monkeypatch.undo()
+    small = c.run(**few).clone()
+    out = torch.zeros_like(small)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.run(**few, out=out)
+    want = c.run().clone()
+    taken = [torch.full((1 << 20,), 77, dtype=torch.uint8, device="cuda") for _ in range(40)]      # what a freed workspace would go to
+    graph.replay()
+    again = c.run()
+    torch.cuda.synchronize()
+    assert torch.equal(out, small) and torch.equal(again, want)
+    assert all(bool((t == 77).all()) for t in taken)
+    c.check(again)
+    c.done()
+
+
 def test_page_offsets_past_32_bits(qm):
     """Pages far into a pool of more than 2^32 elements."""
     import torch

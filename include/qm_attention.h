@@ -442,7 +442,7 @@ int32_t qm_gate_up_swiglu_rows(qm_kv_pool* pool, const uint16_t* x, const uint16
  *   out[r][n] = bf16( float(sum_k x[r][k] * weight[n][k]) * x_scale[r] * weight_scale[n] + bias[n] + residual[r][n] )
  * with one rounding at the end.  qm_quantize_rows_int8 makes both operands (a weight matrix is a matrix of rows too).
  * Rows up to 2^31 - 256: up to 64 go through a split-K cluster kernel, more through persistent 128-row tiles.
- * in_features a multiple of 16, at most 65536; any out_features.  Tensors 16-byte aligned, x_scale 4-byte aligned;
+ * in_features a multiple of 16, at most 65536; any out_features up to 2^31 - 256.  Tensors 16-byte aligned, x_scale 4-byte aligned;
  * bias and residual may be NULL.  The pool's device must be the current device. */
 
 /* scale[r] = max_k |v[r][k]| / 127 and q[r][k] = v[r][k] / scale[r] to the nearest whole number, ties to even, where v

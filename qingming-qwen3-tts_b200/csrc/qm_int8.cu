@@ -26,7 +26,7 @@ namespace {
 constexpr int kQuantThreads = 256;             // CTA per row
 constexpr int kQuantWarps = 8;                 // warp per row
 constexpr int kQuantMaxDim = 24 * 1024;        // the row is staged in shared memory as bf16
-constexpr int kMaxRows = 0x7fffff00;           // a row number rounded up to the next tile is an int too
+constexpr int kMaxRows = 0x7fffff00;           // a row number rounded up to the next tile is an int too (rows of x and of weights)
 
 // With a norm weight the value quantised is v[k] = x[k] * w[k] / rms; the rms divides out of q (q is a ratio of two such
 // values) and enters the scale alone, so one sweep collects both the sum of squares and the largest |x w|, and x w is
@@ -788,7 +788,7 @@ int32_t launch_rows(const int8_t* x, const int8_t* w0, const int8_t* w1, Int8Arg
     if (rc != QM_OK) return rc;
     a.n_tiles = (a.out_cols[0] + kCols - 1) / kCols;
     const long long tiles = (long long)a.m_tiles * a.n_tiles;
-    if (tiles > 0x7fffffffLL) return qm_fail(QM_ECAPACITY, "too many output tiles for one launch");
+    if (tiles > kMaxRows) return qm_fail(QM_ECAPACITY, "too many output tiles for one launch");
     auto kernel = qm_rows_int8_kernel<kBN, kGated>;
     const size_t smem = RowsSmem<kBN>::kTotal + 1024;
     static thread_local int known_device = -1;
@@ -808,7 +808,8 @@ int32_t run_int8(qm_kv_pool* pool, const int8_t* x, const float* x_scale, const 
     if (k_dim < 16 || k_dim % 16 != 0 || k_dim > 65536)
         return qm_fail(QM_EINVAL, "reduction width must be a positive multiple of 16, at most 65536");
     for (int i = 0; i < n_segs; ++i)
-        if (segs[i].out_cols < 1) return qm_fail(QM_EINVAL, "output width must be positive");
+        if (segs[i].out_cols < 1 || segs[i].out_cols > kMaxRows)
+            return qm_fail(QM_EINVAL, "output width must be positive and at most 2^31 - 256");
     if (rows == 0) return QM_OK;                      // nothing to do; the row tensors may then be null
     if (!x || !x_scale || (kGated && (!up || !up_scale))) return qm_fail(QM_EINVAL, "null tensor pointer");
     uintptr_t all = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(up) | reinterpret_cast<uintptr_t>(up_scale) |

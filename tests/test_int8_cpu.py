@@ -59,5 +59,6 @@ def test_quantiser_refuses(qm):
 def test_a_row_number_past_the_last_tile_would_not_fit_an_int(qm):
     lib, p = qm.load_library(), POINTER
     for rows in (2 ** 31 - 1, 2 ** 31 - 255):
+        assert linear(qm, outer=rows) == qm.QM_EINVAL and b"output width" in lib.qm_last_error_string()
         assert linear(qm, rows=rows) == qm.QM_EINVAL and b"rows" in lib.qm_last_error_string()
         assert lib.qm_quantize_rows_int8(p, None, 1e-6, p, p, rows, 64, None) == qm.QM_EINVAL

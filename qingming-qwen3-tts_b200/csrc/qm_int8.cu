@@ -485,7 +485,7 @@ qm_skinny_int8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_co
 // at small K, by the epilogue: 97 us = 2570 Tops for 9923 x 2048 x 6144, 187 us = 2940 Tops for 16384 x 4096 x 4096 (0.77
 // and 0.88 of twice the measured bf16 rate).  Four epilogue warps with scattered 16-byte stores and the column scales
 // read from global memory took 181 and 258 us.  Pairs of SMs on one tile of 256 x 256 (32 KB of operands instead of 48) gain
-// 1 to 3 % above 9000 rows, where the chip's power limit is near, and lose 6 % between 1500 and 4000 rows to their longer
+// 1 to 4 % above 9000 rows, where the chip's power limit is near (114.7 instead of 97 us after 0.3 s of such launches), and lose 6 % between 1500 and 4000 rows to their longer
 // start and end; walking the tiles in groups of 4 to 16 rows of tiles changes neither.
 constexpr int kRowsThreads = 320;              // warps 0-7 epilogue, warp 8 MMA issue, warp 9 TMA loads
 constexpr int kRowsEpilogue = 256;

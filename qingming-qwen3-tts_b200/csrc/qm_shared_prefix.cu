@@ -11,8 +11,8 @@
 // a few dozen pieces of the shared part and one of its own, a CTA per pair of rows with its loads in flight together.
 //
 // Measured (8 KV heads): 64 streams behind 2048 tokens, up to 1024 of their own, 41-43 us (151 MB, 3.6 TB/s;
-// qm_decode_attention 100 us); 83 streams behind five prefixes of up to 4288 tokens, 48 us (184 us); 32 streams behind 32 768
-// tokens, 55 us (204 MB, 3.7 TB/s; 580 us).  What is left above the bytes' 22 to 31 us: about 3 us of plan, 4 us until the
+// qm_decode_attention 100 us); 83 streams behind five prefixes of up to 4288 tokens, 44-48 us (184 us); 32 streams behind 32 768
+// tokens, 52-55 us (204 MB, 3.7 TB/s; 580 us).  What is left above the bytes' 22 to 31 us: about 3 us of plan, 4 us until the
 // first products, 6 us of fold, and CTAs with equal shares that end up to 10 us apart.
 #include "qm_shared_prefix.cuh"
 

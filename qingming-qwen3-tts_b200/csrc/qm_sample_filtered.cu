@@ -85,6 +85,11 @@ struct Smem {
     uint32_t before_count, bin;
 };
 
+__device__ __forceinline__ float fmin3(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ void st_cluster_u64(uint32_t addr, u64 v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
@@ -117,7 +122,8 @@ __device__ __forceinline__ int key_index(u64 key) { return kMaxVocab - 1 - (int)
 // 2^45 exp((x - top) / T):  e = (x - top) / T = k ln2 / 16 + r with |r| <= ln2 / 32; 2^(k / 16) from a table, exp(r) by the first
 // six terms of its series (the seventh is below 2e-13).  A float becomes a double by moving its fields, which is a third of
 // the time of a conversion and takes a zero or a subnormal for a number below 2^-126; where T is so small that this could
-// be seen, by conversion.  For NaN and infinities the result means nothing: callers compare with the cutoff.
+// be seen, by conversion.  For NaN, infinities and scores below the cutoff the result means nothing: callers compare with it (above it e > -66, where
+// the exponent's field cannot wrap, and below -31.9 the weight is less than half of 2^-45 and rounds to zero).
 struct Weigher {
     const double* table;
     double top, inverse;         // 1 / T
@@ -136,8 +142,7 @@ struct Weigher {
         p = fma(p, r, 1.0);
         p = fma(p, r, 1.0);
         p *= table[k & (kTable - 1)];
-        const double w = __hiloint2double(__double2hiint(p) + (k >> 4) * (1 << 20), __double2loint(p));
-        return e > -31.9 ? w : 0.0;                               // below: less than half of 2^-45
+        return __hiloint2double(__double2hiint(p) + (k >> 4) * (1 << 20), __double2loint(p));
     }
     __device__ __forceinline__ double common(float x) const {
         const uint32_t bits = __float_as_uint(x);
@@ -241,13 +246,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
 
     // ---- the largest score and the lowest above -inf, of the row
     float top = -CUDART_INF_F, lowest = CUDART_INF_F;
-    sweep([&](int, int, const Eight& e) {
+    sweep([&](int, int, const Eight& e) {         // neither is ever NaN
+        float low = CUDART_INF_F;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float x = score(e, j);
-            top = fmaxf(top, x);                  // never NaN
-            lowest = fminf(lowest, x > -CUDART_INF_F ? x : CUDART_INF_F);
+        for (int j = 0; j < 8; j += 2) {
+            top = fmax3(top, score(e, j), score(e, j + 1));
+            low = fmin3(low, score(e, j), score(e, j + 1));
         }
+        if (low == -CUDART_INF_F) {
+            low = CUDART_INF_F;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) low = fminf(low, score(e, j) > -CUDART_INF_F ? score(e, j) : CUDART_INF_F);
+        }
+        lowest = fminf(lowest, low);
     });
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) {
@@ -311,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
     // Bins even in z between the largest score and the lowest one that can matter.  Each operation is monotone, so a larger
     // score never has a larger bin; NaN (equal infinities, 0 * inf) comes only where all entries in question are equal or
     // the last of all, and is the last bin.
-    const float per_bin = (float)kBins / fminf(top - lowest, 32.0f * temperature);
+    const float range = fminf(top - lowest, 32.0f * temperature), per_bin = (float)kBins / range;
     auto bin_of = [&](float x) {
         return (int)(__float_as_uint(fminf((top - x) * per_bin, (float)(kBins - 1)) + 8388608.0f) & (kBins - 1));
     };
@@ -487,8 +498,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
                 prefix |= (u64)(kBins - 1 - (int)s.bin) << next;
                 shift = next;
             }
-            // the bin's entries, from all CTAs into all CTAs, if the list holds them
+            // the bin's entries, from all CTAs into all CTAs, if the list holds them; most scores are ruled out by an interval
+            // a hundredth of a bin wider than the bin on either side (bin_of's roundings are a ten-thousandth)
+            float from = cutoff, to = CUDART_INF_F;
+            if (per_bin > 0.0f && per_bin < CUDART_INF_F) {
+                const double width = (double)range * (1.0 / kBins);
+                if (bin < kBins - 1) from = fmaxf(from, __double2float_rd((double)top - ((double)bin + 0.51) * width));
+                to = __double2float_ru((double)top - ((double)bin - 0.51) * width);
+                if (!(to == to)) to = CUDART_INF_F;          // an infinite top or range
+            }
             sweep([&](int, int i0, const Eight& e) {
+                bool near = false;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) near |= score(e, j) >= from && score(e, j) <= to;
+                if (!near) return;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     if (!matches(score(e, j), i0 + j)) continue;
@@ -511,16 +534,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
         }
         __syncthreads();
         // rank by counting: what the larger keys measure
-        u64 last = ~0ull;
-        for (int e = tid; e < found; e += kThreads) {
-            const u64 key = s.all[e].x;
-            u64 before = by_mass ? ahead_mass : (u64)ahead_count;
+        u64 last = ~0ull, keys[2], before[2];     // two entries per thread at most
+        static_assert(kList == 2 * kThreads, "entries per thread");
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            keys[e] = tid + e * kThreads < found ? s.all[tid + e * kThreads].x : ~0ull;
+            before[e] = by_mass ? ahead_mass : (u64)ahead_count;
+        }
+        if (tid < found)
             for (int j = 0; j < found; ++j) {
                 const ulonglong2 other = s.all[j];
-                before += other.x > key ? other.y : 0ull;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) before[e] += other.x > keys[e] ? other.y : 0ull;
             }
-            if (before < limit && key < last) last = key;
-        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (before[e] < limit && keys[e] < last) last = keys[e];
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) {
             const u64 other = __shfl_xor_sync(0xffffffffu, last, off);
@@ -545,6 +574,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
 
     // ---- the draw: kept weights in index order, summed by blocks (the bins' place is free again)
     const u64 least = min_p > 0.0f ? (u64)ceil((double)fminf(min_p, 2.0f) * kUnit) : 0ull;
+    // a score below this is out; above it min-p is compared exactly (the margin is far above the errors of logf, and of the
+    // weights' own rounding where min_p is not tiny)
+    float bound = cutoff;
+    if (min_p >= 1.0e-6f) bound = fmaxf(bound, fminf(top, __double2float_rd((double)top + (double)temperature * ((double)logf(min_p) - 1.0e-4))));
+    bound = fmaxf(bound, threshold);
     const bool filtered = threshold > -CUDART_INF_F || least > 0ull;
     auto stays_in = [&](float x, int i) { return x >= cutoff && stays(x, i); };
     auto kept = [&](float x, int i) -> u64 {
@@ -565,22 +599,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum += score(e, j) >= cutoff ? q[j] : 0ull;
         } else {
-            // mostly few of the 256: side by side first, then a weight per lane
-            uint32_t mine = 0;
+            uint32_t in = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) mine |= score(e, j) >= threshold ? 1u << j : 0u;
-            if (!__any_sync(0xffffffffu, mine != 0u)) {
+            for (int j = 0; j < 8; ++j) in |= score(e, j) >= bound ? 1u << j : 0u;
+            if (!__any_sync(0xffffffffu, in != 0u)) {
                 if (lane == 0) block_sum[block] = 0ull;
                 return;
             }
-            mine = 0;
+            // at the threshold itself the index decides
 #pragma unroll
-            for (int j = 0; j < 8; ++j) mine |= stays_in(score(e, j), i0 + j) ? 1u << j : 0u;
-            const int upto = warp_inclusive(__popc(mine), lane), count = __shfl_sync(0xffffffffu, upto, 31);
-            int at = upto - __popc(mine);
+            for (int j = 0; j < 8; ++j) in &= score(e, j) != threshold || i0 + j <= threshold_index ? 0xffu : ~(1u << j);
+            const int upto = warp_inclusive(__popc(in), lane), count = __shfl_sync(0xffffffffu, upto, 31);
+            // side by side first, then a weight per lane (weighing all eight in place from 32, 64 or 128 of the 256 on: no faster)
+            int at = upto - __popc(in);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (mine >> j & 1u) few[at++] = score(e, j);
+                if (in >> j & 1u) few[at++] = score(e, j);
             __syncwarp();
             for (int i = lane; i < count; i += 32) {
                 const float x = few[i];

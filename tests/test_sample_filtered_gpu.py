@@ -153,6 +153,25 @@ def test_the_ends_of_the_parameters(eng):
     assert bool((t == 17).all()), "a NaN temperature is greedy, the lower of two equal scores wins"
 
 
+@pytest.mark.parametrize("offset", [0.0, 3.0e4, -1.0e5, 1.0e30, -1.0e-30])
+@pytest.mark.parametrize("vocab", [700, 20000])
+def test_scores_far_from_zero(eng, offset, vocab):
+    """Scores whose spacing is near a bin's width, a temperature's, or min-p's border, with a min-p at either side of 1e-6."""
+    import torch
+
+    z = offset + scores(31, 12, vocab, 3.0) * max(1.0, abs(offset) * 2.0 ** -20)
+    if abs(offset) < 1e-20:
+        z = z * 1e-30
+    size = float(z.amax() - z.amin())
+    for seed, share in enumerate((1e-6, 1e-3, 0.1, 1.0, 100.0)):
+        heat = [max(size * share * f, 1e-38) for f in (0.3, 0.7, 1.0)] * 4
+        u = uniform(seed, 12)
+        check(eng, z, u, heat=heat, low=[1.0, 0.5, 0.1, 1e-3, 1.0001e-6, 0.999e-6, 1e-9, 1e-20, 0.9999999, 3.0, 0.25, 0.0])
+        check(eng, z, u, heat=heat, p=[0.2, 0.9, 0.999, 0.6] * 3, k=[0, 100, 500, 7] * 3)
+    flat = torch.full((2, vocab), offset, device="cuda")
+    check(eng, flat, [0.3, 0.9], p=[0.4, 1.0], low=[1.0, 0.5])
+
+
 def test_strides_offsets_and_types(eng):
     import torch
 

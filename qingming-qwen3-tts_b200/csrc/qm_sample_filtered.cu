@@ -18,13 +18,15 @@
 // A row is spread over a cluster of up to eight CTAs; the scores come from the L2 for every sweep after the first.
 // Nothing is sorted as a whole: a sweep puts the entries (for top-p their weights too) into 1024 bins that are even in z,
 // the CTAs add their bins up, a slice of them each, and every CTA finds the bin in which top-k (or top-p) ends by the
-// same scan.  The few entries of that bin are gathered and ranked by counting.  A bin with more than 512 entries
-// (many equal scores) is first cut down by digits of the entries' keys, which contain the index and therefore differ.
+// same scan.  The few entries of that bin are gathered and put in order.  A bin with more than 512 entries
+// (many equal scores) is first cut down by digits of the entries' keys, which contain the index and therefore differ.  Where
+// top-k leaves few entries, they are gathered as a whole, and top-p, min-p and the draw need no sweep any more.
 // What bounds it: instructions (a weight is about 40, twelve of them in double precision; a top-p row of a large vocabulary
-// about 160 per score in all) and, for small rows, the steps' latency.  Measured: one row of 2048 with top-k 8.3 us, 64
-// rows of 2048 with everything 14 us, 32 rows of 131 072 fp32 50 us, 96 rows of 100 003 bf16 29 us without filters, 38 us with
-// top-k, 92 us with top-p.  Tried and slower: the scores kept in shared memory (196 us; fewer CTAs fit), clusters of three
-// with two CTAs on every SM (125 us), 512 threads per CTA (103 us, though 45 us at 131 072).
+// about 130 per score in all) and, for small rows, the steps' latency.  Measured: one row of 2048 with top-k 6.7 us, 64
+// rows of 2048 with everything 12 us, 32 rows of 131 072 fp32 45-52 us, 96 rows of 100 003 bf16 28 us without filters, 27 us
+// with top-k 50 (and top-p and min-p behind it), 18 us with min-p, 81 us with top-p 0.7 to 1.  Tried and slower, when that took
+// 92: the scores kept in shared memory (196 us; fewer CTAs fit), clusters of three with two CTAs on every SM (125 us), 512
+// threads per CTA (103 us, though 45 instead of 50 us at 131 072).
 #include <math_constants.h>
 
 #include <cfloat>
@@ -82,7 +84,7 @@ struct Smem {
     uint32_t found;
     // the chosen bin
     u64 before_mass;
-    uint32_t before_count, bin;
+    uint32_t before_count, upto_count, bin;
 };
 
 __device__ __forceinline__ float fmin3(float a, float b, float c) {
@@ -340,9 +342,98 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
     int threshold_index = -1;                     // (of the slice)
     auto stays = [&](float x, int i) { return x > threshold || (x == threshold && i <= threshold_index); };
 
+    // The first n entries of s.all into descending order of key & mask, by a bitonic network over the next power of two (returned;
+    // what is behind the entries is zero).  A warp's pairs at distances up to 32 lie in 64 entries of its own.
+    auto sort_list = [&](int n, u64 mask) {
+        int size_all = 64;
+        while (size_all < n) size_all *= 2;
+        __syncthreads();
+        for (int i = n + tid; i < size_all; i += kThreads) s.all[i] = make_ulonglong2(0ull, 0ull);      // behind every entry
+        __syncthreads();
+        for (int size = 2; size <= size_all; size *= 2) {
+            for (int stride = size / 2; stride > 0; stride /= 2) {
+                if (tid < size_all / 2) {
+                    const int lo = 2 * tid - (tid & (stride - 1)), hi = lo + stride;
+                    const ulonglong2 x = s.all[lo], y = s.all[hi];
+                    if (((x.x & mask) < (y.x & mask)) == ((lo & size) == 0)) {
+                        s.all[lo] = y;
+                        s.all[hi] = x;
+                    }
+                }
+                if (stride > 32 || (stride == 1 && size >= 64)) __syncthreads();
+                else __syncwarp();
+            }
+        }
+        return size_all;
+    };
+    // Sum over the block of a value of every thread, and of the threads before this one.
+    auto scan_block = [&](u64 v, u64& total) {
+        const u64 to = warp_inclusive(v, lane);
+        __syncthreads();
+        if (lane == 31) s.scan_mass[warp] = to;
+        __syncthreads();
+        u64 ahead = to - v;
+        total = 0ull;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            ahead += w < warp ? s.scan_mass[w] : 0ull;
+            total += s.scan_mass[w];
+        }
+        return ahead;
+    };
+    // The first n entries of s.all in descending order of key & mask: every entry, its place in the order and the weight in front of
+    // it in some thread (two at most).  Up to 128 entries stay where they are and are counted, two to eight threads to an
+    // entry; more are sorted.  Measured: a row of 2048 with top-k 50 counted 6.1, sorted 10.2 us; 96 rows with some 300 entries
+    // at top-p's border counted 94, sorted 81 us (rows with 200 entries for top-k 43.7 and 39.4 us).
+    struct Ordered {
+        u64 key[2], weight[2], ahead[2];          // none: key ~0, weight 0
+        int place[2], slot[2];                    // slot in s.all, or -1
+    };
+    auto order_list = [&](int n, u64 mask, Ordered& o) {
+        u64 total;
+        if (n > kThreads / 2) {
+            const int sorted = sort_list(n, mask);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                o.slot[e] = o.place[e] = 2 * tid + e;
+                const ulonglong2 entry = o.slot[e] < sorted ? s.all[o.slot[e]] : make_ulonglong2(0ull, 0ull);
+                if (entry.x == 0ull) o.slot[e] = -1;
+                o.key[e] = entry.x == 0ull ? ~0ull : entry.x;
+                o.weight[e] = entry.y;
+            }
+            o.ahead[0] = scan_block(o.weight[0] + o.weight[1], total);
+            o.ahead[1] = o.ahead[0] + o.weight[0];
+            return total;
+        }
+        const int t = n <= kThreads / 8 ? 8 : (n <= kThreads / 4 ? 4 : 2), i = tid / t;
+        const u64 key = i < n ? s.all[i].x : ~0ull;
+        u64 ahead = 0ull;
+        int place = 0;
+#pragma unroll 4
+        for (int j = tid & (t - 1); j < n; j += t) {
+            const ulonglong2 other = s.all[j];
+            const bool before = (other.x & mask) > (key & mask);
+            place += before ? 1 : 0;
+            ahead += before ? other.y : 0ull;
+        }
+        for (int off = 1; off < t; off <<= 1) {
+            place += __shfl_xor_sync(0xffffffffu, place, off);
+            ahead += __shfl_xor_sync(0xffffffffu, ahead, off);
+        }
+        const bool mine = i < n && (tid & (t - 1)) == 0;
+        o = {{mine ? key : ~0ull, ~0ull}, {mine ? s.all[i].y : 0ull, 0ull}, {ahead, 0ull}, {place, 0}, {mine ? i : -1, -1}};
+        scan_block(o.weight[0], total);
+        return total;
+    };
+    static_assert(kList == 2 * kThreads, "two entries per thread");
+
     // The last entry of the order, among those that stay so far, whose predecessors count less than k (by_mass false) or
     // weigh less than p times all of them: the new threshold.
-    auto search = [&](bool by_mass, int k, float p, bool bins_are_clear) {
+    // For a count, where the bin and all before it are few, they are listed (keys and weights, in the first CTA) and the rest
+    // of the row's work is done there: returns their number, otherwise 0.  Few: what the list holds if p < 1, which saves the
+    // sweeps of that search (96 rows of 100 003, top-k 200 and top-p 65.6 -> 40 us), otherwise what is counted and not
+    // sorted (top-k 50 32.3 -> 26.5 us; for 200 the sweep of the draw takes 36.5 us, sorting 40).
+    auto search = [&](bool by_mass, int k, float p, bool bins_are_clear) -> int {
         int shift = 64, bin = 0;                  // from the second round on: the chosen bin, keys that agree with prefix above `shift`
         u64 prefix = 0ull, limit = (u64)k;
         uint32_t ahead_count = 0;
@@ -470,13 +561,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
                 limit = wanted > 1.0 ? (u64)wanted : 1ull;
             }
             int mine = -1;
-            uint32_t my_count = 0;
+            uint32_t my_count = 0, my_upto = 0;
             u64 my_mass = 0;
 #pragma unroll
             for (int j = 0; j < kBinsPerThread; ++j) {
                 if ((by_mass ? m[j] != 0ull && mb < limit : c[j] != 0u && (u64)cb < limit)) {
                     mine = tid * kBinsPerThread + j;
                     my_count = cb;
+                    my_upto = cb + c[j];
                     my_mass = mb;
                 }
                 cb += c[j];
@@ -487,6 +579,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
             if (mine >= 0 && s.found == (uint32_t)mine + 1u) {
                 s.bin = (uint32_t)mine;
                 s.before_count = my_count;
+                s.upto_count = my_upto;
                 s.before_mass = my_mass;
             }
             __syncthreads();
@@ -501,10 +594,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
             // the bin's entries, from all CTAs into all CTAs, if the list holds them; most scores are ruled out by an interval
             // a hundredth of a bin wider than the bin on either side (bin_of's roundings are a ten-thousandth)
             float from = cutoff, to = CUDART_INF_F;
+            const bool list_all = !by_mass && round == 0 && s.upto_count <= (uint32_t)(p < 1.0f ? kList : kThreads / 2);
             if (per_bin > 0.0f && per_bin < CUDART_INF_F) {
                 const double width = (double)range * (1.0 / kBins);
                 if (bin < kBins - 1) from = fmaxf(from, __double2float_rd((double)top - ((double)bin + 0.51) * width));
-                to = __double2float_ru((double)top - ((double)bin - 0.51) * width);
+                if (!list_all) to = __double2float_ru((double)top - ((double)bin - 0.51) * width);
                 if (!(to == to)) to = CUDART_INF_F;          // an infinite top or range
             }
             sweep([&](int, int i0, const Eight& e) {
@@ -514,42 +608,33 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
                 if (!near) return;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    if (!matches(score(e, j), i0 + j)) continue;
+                    const float x = score(e, j);
+                    if (list_all ? !(x >= cutoff) || bin_of(x) > bin : !matches(x, i0 + j)) continue;
                     const uint32_t at = atomicAdd(&s.list_count, 1u);
-                    if (at < kList) s.list[at] = entry_key(score(e, j) + 0.0f, begin + i0 + j);
+                    if (at < kList) s.list[at] = entry_key(x + 0.0f, begin + i0 + j);
                 }
             });
             sync_all();
             found = 0;
-            for (int r = 0; r < cluster; ++r) {
+            for (int r = 0; r < cluster && (!list_all || rank == 0); ++r) {
                 const int there = (int)(cluster > 1 ? ld_cluster_u32(remote(&s.list_count, r)) : s.list_count);
                 for (int i = tid; i < there && found + i < kList; i += kThreads) {
                     const u64 key = cluster > 1 ? ld_cluster_u64(remote(&s.list[i], r)) : s.list[i];
-                    s.all[found + i] = make_ulonglong2(key, by_mass ? whole(weight(key_score(key))) : 1ull);
+                    s.all[found + i] = make_ulonglong2(key, by_mass || list_all ? whole(weight(key_score(key))) : 1ull);
                 }
                 found += there;
             }
+            if (list_all) return (int)s.upto_count;
             if (found <= kList) break;
             sync_all();                           // the others' lists have been looked at
         }
         __syncthreads();
-        // rank by counting: what the larger keys measure
-        u64 last = ~0ull, keys[2], before[2];     // two entries per thread at most
-        static_assert(kList == 2 * kThreads, "entries per thread");
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            keys[e] = tid + e * kThreads < found ? s.all[tid + e * kThreads].x : ~0ull;
-            before[e] = by_mass ? ahead_mass : (u64)ahead_count;
-        }
-        if (tid < found)
-            for (int j = 0; j < found; ++j) {
-                const ulonglong2 other = s.all[j];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) before[e] += other.x > keys[e] ? other.y : 0ull;
-            }
+        Ordered o;
+        order_list(found, ~0ull, o);
+        u64 last = ~0ull;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-            if (before[e] < limit && keys[e] < last) last = keys[e];
+            if (o.ahead[e] + (by_mass ? ahead_mass : (u64)ahead_count) < limit && o.key[e] < last) last = o.key[e];
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) {
             const u64 other = __shfl_xor_sync(0xffffffffu, last, off);
@@ -563,17 +648,53 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
         __syncthreads();
         threshold = key_score(last);
         threshold_index = key_index(last) - begin;
+        return 0;
     };
 
     const int k = a.top_k ? a.top_k[row] : 0;
     const float p = a.top_p ? a.top_p[row] : 1.0f;
     const float min_p = a.min_p ? a.min_p[row] : 0.0f;
     const bool cut_k = k > 0 && k < a.vocab;
-    if (cut_k) search(false, k, 1.0f, true);
+    const u64 least = min_p > 0.0f ? (u64)ceil((double)fminf(min_p, 2.0f) * kUnit) : 0ull;
+    const double uniform = (double)a.uniforms[row];
+    auto target_of = [&](u64 total) {
+        const double wanted = uniform * (double)total;
+        const u64 target = wanted > 0.0 ? (wanted < (double)total ? (u64)wanted : total - 1ull) : 0ull;
+        return target < total ? target : total - 1ull;
+    };
+    const int listed = cut_k ? search(false, k, p, true) : 0;
+    if (listed > 0) {
+        // ---- all that can stay is in the first CTA's list: the remaining filters and the draw there
+        sync_all();                               // the list is whole, and nobody's is needed any more
+        if (rank != 0) return;
+        Ordered o;
+        order_list(listed, ~0ull, o);
+        u64 total, sum = 0ull, limit = ~0ull;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) sum += o.place[e] < k ? o.weight[e] : 0ull;
+        scan_block(sum, total);
+        if (p < 1.0f) {
+            const double wanted = ceil((double)p * (double)total);
+            limit = wanted > 1.0 ? (u64)wanted : 1ull;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (o.slot[e] >= 0 && (o.place[e] >= k || o.ahead[e] >= limit || (o.weight[e] < least && key_score(o.key[e]) != top)))
+                s.all[o.slot[e]].y = 0ull;
+        __syncthreads();
+        total = order_list(listed, (u64)(kMaxVocab - 1), o);      // by index
+        const u64 target = target_of(total);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (target >= o.ahead[e] && target < o.ahead[e] + o.weight[e]) {
+                a.tokens[row] = key_index(o.key[e]);
+                if (a.probs) a.probs[row] = (float)(weight(key_score(o.key[e])) / (double)total);
+            }
+        return;
+    }
     if (p < 1.0f) search(true, 0, p, !cut_k);
 
     // ---- the draw: kept weights in index order, summed by blocks (the bins' place is free again)
-    const u64 least = min_p > 0.0f ? (u64)ceil((double)fminf(min_p, 2.0f) * kUnit) : 0ull;
     // a score below this is out; above it min-p is compared exactly (the margin is far above the errors of logf, and of the
     // weights' own rounding where min_p is not tiny)
     float bound = cutoff;
@@ -645,9 +766,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) qm_sample_filtered_kerne
             total += s.totals[r];
         }
     }
-    const double wanted = (double)a.uniforms[row] * (double)total;
-    u64 target = wanted > 0.0 ? (wanted < (double)total ? (u64)wanted : total - 1ull) : 0ull;
-    if (target >= total) target = total - 1ull;
+    const u64 target = target_of(total);
     if (warp > 0 || target < before || target >= before + own) return;
     // The first warp of the CTA that has it: which block, which lane's eight, which of them.
     u64 sum = before;

@@ -153,6 +153,21 @@ def test_the_ends_of_the_parameters(eng):
     assert bool((t == 17).all()), "a NaN temperature is greedy, the lower of two equal scores wins"
 
 
+@pytest.mark.parametrize("vocab", [300, 2048, 40000, 262144])
+@pytest.mark.parametrize("share", [1.0, 0.6])
+def test_top_k_of_every_size(eng, vocab, share):
+    """Around the sizes at which the entries that can stay are sorted as one list, or no longer; the last index among them."""
+    ks = [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200, 255, 256, 257, 400, 480, 500, 511, 512, 513, 600, 1000]
+    n = len(ks)
+    z = scores(41, n, vocab)
+    z[:, vocab - 1] = z.amax(1) - 0.1
+    z[::2, 0] = z[::2].amax(1)
+    for seed in range(3):
+        u = uniform(seed, n) if seed < 2 else [0.99999] * n
+        check(eng, z, u, k=ks, p=[share] * n, low=[0.0, 0.01, 0.2][seed:seed + 1] * n, heat=[1.0, 3.0, 0.5][seed:seed + 1] * n)
+    check(eng, z.round(), uniform(7, n), k=ks, p=[share] * n)
+
+
 @pytest.mark.parametrize("offset", [0.0, 3.0e4, -1.0e5, 1.0e30, -1.0e-30])
 @pytest.mark.parametrize("vocab", [700, 20000])
 def test_scores_far_from_zero(eng, offset, vocab):

@@ -291,7 +291,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
         pdl_wait();
         const int len = word(a.seq_lens, a.batch), start = word(g.starts, g.groups + 1), pages = word(g.pages, g.groups);
         if (__syncthreads_or(len != old_len || start != old_start || pages != old_pages)) plan = make_plan(len, start, pages);
-        if (blockIdx.x == 0) publish_shared_plan(plan, g, a.batch, a.status, tid);
+        if (blockIdx.x == 0) {
+            const int kept = len < 0 ? 0 : (len > cap_len ? cap_len : len);
+            publish_shared_plan(plan, g, tid < a.batch ? units_of(kept) : 0, a.batch, a.status, tid);
+        }
         const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::kFlagOff);
         if (cta < plan.ctas) {
             shared_prefix_role(plan, g, maps.q, maps.k, maps.v, smem, smem_addr(smem + PrefixLayout::kPrefixBarOff), a.page_table,
@@ -330,7 +333,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
         xview = exchange_cache_peers(a.exchange, reinterpret_cast<unsigned char**>(smem + L::kPeerOff), tid);
         __syncthreads();
     }
-    for (int s = cta; s < a.batch; s += ctas) {
+    // With shared prefixes the fold knows who has none.
+    for (int s = cta; !kShared && s < a.batch; s += ctas) {
         if (prefix[s + 1] != prefix[s]) continue;
         if (kExchange) {
             if (tid < kHeadDim) {        // warps 0-3, one row after the other

@@ -45,8 +45,10 @@ __global__ void __launch_bounds__(kCombineThreads) qm_shared_combine_kernel(cons
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int stream = blockIdx.x / kv_heads, head = blockIdx.x - stream * kv_heads;
     const size_t row0 = (size_t)blockIdx.x * 2;
-    const int4 st = __ldcg(reinterpret_cast<const int4*>(g.streams + stream));     // base, splits, group_rows, row
-    // the own part, fetched beside the descriptor
+    int4 st = __ldcg(reinterpret_cast<const int4*>(g.streams + stream));     // base, splits, group_rows, row
+    const bool has_own = (st.w & 1) != 0;
+    st.w &= ~1;
+    // the own part, fetched beside the descriptor; without one the place holds what some earlier call left there
     const float* mine = own + (row0 + (warp & 1)) * kOwnStride;
     const float2 own_ml = __ldcg(reinterpret_cast<const float2*>(mine));
     const float2 own_a = __ldcg(reinterpret_cast<const float2*>(mine + 2 + 4 * lane));
@@ -90,9 +92,9 @@ __global__ void __launch_bounds__(kCombineThreads) qm_shared_combine_kernel(cons
     }
     __syncthreads();
     if (warp < 2) {
-        float top = own_ml.x * kLog2e, sum = own_ml.y;
-        float4 acc = make_float4(own_a.x, own_a.y, own_b.x, own_b.y);
-        bool empty = sum == 0.0f;                 // a stream without keys of its own: m = -inf, l = 0, o = 0
+        float top = own_ml.x * kLog2e, sum = has_own ? own_ml.y : 0.0f;
+        float4 acc = has_own ? make_float4(own_a.x, own_a.y, own_b.x, own_b.y) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        bool empty = !has_own;
 #pragma unroll
         for (int w = 0; w < kCombineWarps; ++w) {
             if (w >= st.y) break;

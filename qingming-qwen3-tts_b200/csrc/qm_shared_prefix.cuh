@@ -26,7 +26,7 @@ struct SharedStream {
     int base;
     int splits;          // 0: nothing shared
     int group_rows;      // 2 * streams of the group
-    int row;             // 2 * place in the group
+    int row;             // 2 * place in the group; + 1: the stream has pages of its own, and so a partial result over them
 };
 
 struct SharedGroups {
@@ -226,8 +226,11 @@ __device__ __forceinline__ SharedPlan make_shared_plan(const SharedGroups& g, in
     return p;
 }
 
-// Where each stream's partial results will lie, for the launch that folds them.  One CTA, once the plan is final.
-__device__ __forceinline__ void publish_shared_plan(const SharedPlan& p, const SharedGroups& g, int batch, uint32_t* status, int tid) {
+// Which partial results each stream will have and where, for the launch that folds them.  One CTA, once the plan is final;
+// own_units: pages x KV heads that are attended for stream `tid` alone.  A stream without any has no partial result of its
+// own, written by nobody (the whole grid may be at shared pieces then): the fold must not read one.
+__device__ __forceinline__ void publish_shared_plan(const SharedPlan& p, const SharedGroups& g, int own_units, int batch, uint32_t* status,
+                                                    int tid) {
     if (tid == 0 && p.words[3]) atomicOr(status, QM_DEVSTAT_BAD_POS);
     if (tid >= batch) return;
     int4 w = make_int4(0, 0, 0, 0);
@@ -235,6 +238,7 @@ __device__ __forceinline__ void publish_shared_plan(const SharedPlan& p, const S
         const int group = group_of_stream(p.starts, g.groups, tid), first = p.starts[group];
         w = make_int4(p.rows[group], (p.pages[group] + p.piece - 1) / p.piece, 2 * (p.starts[group + 1] - first), 2 * (tid - first));
     }
+    if (own_units > 0) w.w += 1;
     *reinterpret_cast<int4*>(g.streams + tid) = w;
 }
 

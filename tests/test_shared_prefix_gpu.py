@@ -317,3 +317,30 @@ def test_the_python_call_checks_its_tensors(qm):
         with pytest.raises(ValueError):
             c.run(**bad)
     c.done()
+
+
+NOBODY = {
+    "as many pieces as CTAs": dict(groups=[(6, 74)]),                        # 8 heads x 37 pieces of two pages: 2 x 148 SMs
+    "as many pieces as CTAs, longer": dict(groups=[(6, 148)]),
+    "pieces go round": dict(groups=[(1, 1 + i % 4) for i in range(50)], kv_heads=9),
+    "few pieces": dict(groups=[(5, 3), (2, 9)], kv_heads=2),
+}
+
+
+@pytest.mark.parametrize("name", list(NOBODY))
+def test_nobody_has_keys_of_its_own_after_a_call_where_everybody_had(qm, name):
+    """Lengths that end with the shared part, or at nothing: what an earlier call left in the workspace is not folded in."""
+    import torch
+
+    c = Case(qm, own=[70, 5], seed=30 + len(name), **NOBODY[name])
+    before = c.run().clone()
+    c.check(before)
+    shared = [p * PAGE for n, p in NOBODY[name]["groups"] for _ in range(n)]
+    for idle in (10 ** 6, 3):
+        lens = [0 if i % idle == 1 else n for i, n in enumerate(shared)]
+        seq = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        first = c.run(seq_lens=seq).clone()
+        c.check(first, lens=lens)
+        assert torch.equal(c.run(), before)
+        assert torch.equal(c.run(seq_lens=seq), first)
+    c.done()

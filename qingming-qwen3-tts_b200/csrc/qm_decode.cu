@@ -292,8 +292,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
         const int len = word(a.seq_lens, a.batch), start = word(g.starts, g.groups + 1), pages = word(g.pages, g.groups);
         if (__syncthreads_or(len != old_len || start != old_start || pages != old_pages)) plan = make_plan(len, start, pages);
         if (blockIdx.x == 0) {
-            const int kept = len < 0 ? 0 : (len > cap_len ? cap_len : len);
-            publish_shared_plan(plan, g, tid < a.batch ? units_of(kept) : 0, a.batch, a.status, tid);
+            // lengths are reported here: there may be no CTA below that looks at them
+            publish_shared_plan(plan, g, tid < a.batch ? units_of(clamp_len(len, a.max_pages, a.status)) : 0, a.batch, a.status, tid);
         }
         const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::kFlagOff);
         if (cta < plan.ctas) {

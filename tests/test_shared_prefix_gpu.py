@@ -344,3 +344,22 @@ def test_nobody_has_keys_of_its_own_after_a_call_where_everybody_had(qm, name):
         assert torch.equal(c.run(), before)
         assert torch.equal(c.run(seq_lens=seq), first)
     c.done()
+
+
+@pytest.mark.parametrize("pages", [74, 75])
+def test_a_length_past_the_table_is_reported_whichever_ctas_run(qm, pages):
+    """Tables that end with the shared part: a longer stream is cut to it, and nobody has keys of its own."""
+    import torch
+
+    c = Case(qm, [(6, pages)], [0], seed=31)
+    table = c.table[:, :pages].contiguous()
+    want = c.run(page_table=table).clone()
+    assert c.eng.status() == 0
+    c.check(want)
+    over = c.seq.clone()
+    over[2] += 1
+    assert torch.equal(c.run(page_table=table, seq_lens=over), want)
+    assert c.eng.status() == qm.DEVSTAT_BAD_POS
+    assert torch.equal(c.run(page_table=table, seq_lens=torch.full_like(c.seq, 2 ** 31 - 1)), want)
+    assert c.eng.status() == qm.DEVSTAT_BAD_POS
+    c.done()

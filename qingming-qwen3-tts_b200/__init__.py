@@ -320,9 +320,12 @@ class TalkerAttention:
         if ws is None:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the first launch_attention_shared makes its workspace and cannot be captured")
+            if dev != self.rope_cos.get_device():
+                raise QmError(QM_EINVAL, "the pool's device must be the current device")
             need = self.lib.qm_decode_shared_workspace_bytes(self.pool, SHARED_MAX_BATCH)
-            self._shared_workspace = ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+            ws = torch.empty(need, dtype=torch.uint8, device="cuda")
             _check(self.lib.qm_decode_workspace_init(_ptr(ws), need, _stream()))
+            self._shared_workspace = ws          # only once it is on the pool's device and prepared: later calls rely on it
         _check(self.lib.qm_decode_attention_shared(
             self.pool, layer, _need("q_rot", q_rot, bf16, dev, batch, self.q_heads, HEAD_DIM), _need("seq_lens", seq_lens, i32, dev, batch),
             _need("page_table", page_table, i32, dev, batch, max_pages), max_pages, batch, self.q_heads,

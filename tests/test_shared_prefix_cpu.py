@@ -44,3 +44,90 @@ def test_workspace_covers_the_plain_call_and_the_pieces(qm):
     for batch in (1, 64, 256):
         need = lib.qm_decode_shared_workspace_bytes(pool, batch)
         assert need >= lib.qm_decode_workspace_bytes(batch, 8) + 2 * 148 * 128 * 520
+
+
+class Tensor:
+    """What the Python call looks at in a tensor."""
+
+    def __init__(self, dtype, *shape, device=0):
+        self.dtype, self.shape, self.device = dtype, shape, device
+
+    def get_device(self):
+        return self.device
+
+    def is_contiguous(self):
+        return True
+
+    def numel(self):
+        return 1 << 30
+
+    def data_ptr(self):
+        return P
+
+    def stride(self):
+        return ()
+
+
+class Library:
+    """Counts the workspaces it is asked to prepare; `init` and `launch` are what those calls answer."""
+
+    def __init__(self, init, launch):
+        self.prepared, self.init, self.launch = 0, init, launch
+
+    def qm_decode_shared_workspace_bytes(self, pool, batch):
+        return 64
+
+    def qm_decode_workspace_init(self, workspace, size, stream):
+        self.prepared += 1
+        return self.init
+
+    def qm_decode_attention_shared(self, *args):
+        return self.launch
+
+
+def python_call(qm, monkeypatch, library, pool_device=0, device=0, seq_lens=3):
+    import torch
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch, "empty", lambda *size, **kw: Tensor(torch.uint8, device=device))
+    monkeypatch.setattr(qm, "_stream", lambda: 0)
+    eng = object.__new__(qm.TalkerAttention)
+    eng.lib, eng.pool, eng.q_heads, eng.kv_heads, eng._shared_workspace = library, None, 4, 2, None
+    eng.rope_cos = Tensor(torch.bfloat16, 1, 128, device=pool_device)
+    bf16, i32 = torch.bfloat16, torch.int32
+
+    def call():
+        q = Tensor(bf16, 3, 4, 128, device=device)
+        return eng.launch_attention_shared(0, q, Tensor(i32, seq_lens, device=device), Tensor(i32, 3, 5, device=device),
+                                           Tensor(i32, 2, device=device), Tensor(i32, 1, device=device), 2, out=q)
+    return eng, call
+
+
+def test_the_python_call_makes_its_workspace_once(qm, monkeypatch):
+    library = Library(qm.QM_OK, qm.QM_OK)
+    eng, call = python_call(qm, monkeypatch, library)
+    call()
+    first = eng._shared_workspace
+    call()
+    assert first is not None and eng._shared_workspace is first and library.prepared == 1
+
+
+def test_a_call_from_another_device_leaves_no_workspace_there(qm, monkeypatch):
+    """The pool is on device 0 and device 1 is current: later calls on device 0 must not be given memory of device 1."""
+    library = Library(qm.QM_OK, qm.QM_EINVAL)
+    eng, call = python_call(qm, monkeypatch, library, pool_device=0, device=1)
+    with pytest.raises(qm.QmError):
+        call()
+    assert eng._shared_workspace is None and library.prepared == 0
+
+
+def test_a_workspace_that_could_not_be_prepared_is_not_kept(qm, monkeypatch):
+    library = Library(qm.QM_ECUDA, qm.QM_OK)
+    eng, call = python_call(qm, monkeypatch, library)
+    with pytest.raises(qm.QmError):
+        call()
+    assert eng._shared_workspace is None
+    library.init = qm.QM_OK
+    call()
+    assert eng._shared_workspace is not None and library.prepared == 2

@@ -159,6 +159,7 @@ int32_t qm_decode_attention_shared(qm_kv_pool* pool, int32_t layer, const uint16
     if (batch < 0 || max_pages < 1 || groups < 0 || max_shared_pages < 0) return qm_fail(QM_EINVAL, "invalid geometry");
     if (batch > kSharedMaxBatch || groups > kSharedMaxBatch)
         return qm_fail(QM_ECAPACITY, "shared-prefix attention takes at most 256 streams and 256 groups per call");
+    if (batch == 0) return QM_OK;                     // nothing to do; the tensors may then be null
     if (!q_rot || !seq_lens || !page_table || !out || !workspace || (groups > 0 && (!group_starts || !shared_pages)))
         return qm_fail(QM_EINVAL, "null tensor pointer");
     if ((reinterpret_cast<uintptr_t>(q_rot) & 15u) || (reinterpret_cast<uintptr_t>(workspace) & 15u) ||
@@ -166,7 +167,6 @@ int32_t qm_decode_attention_shared(qm_kv_pool* pool, int32_t layer, const uint16
         return qm_fail(QM_EINVAL, "q_rot and workspace must be 16-byte aligned, out 8-byte aligned");
     if (workspace_bytes < qm_decode_shared_workspace_bytes(pool, batch))
         return qm_fail(QM_EINVAL, "workspace smaller than qm_decode_shared_workspace_bytes()");
-    if (batch == 0) return QM_OK;
     int device = -1;
     QM_CUDA_TRY(cudaGetDevice(&device), "get current device");
     if (device != pool->device) return qm_fail(QM_EINVAL, "the pool's device must be the current device");

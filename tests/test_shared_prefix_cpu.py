@@ -37,6 +37,13 @@ def test_an_empty_batch_is_no_work(qm):
     assert shared(qm, batch=0) == qm.QM_OK
 
 
+def test_the_tensors_of_an_empty_batch_may_be_null(qm):
+    """An empty PyTorch tensor has no address."""
+    assert shared(qm, batch=0, q=None, lens=None, table=None, out=None, starts=None, pages=None, groups=0) == qm.QM_OK
+    assert shared(qm, batch=0, q=None, lens=None, table=None, out=None) == qm.QM_OK
+    assert shared(qm, batch=0, layer=2, q=None) == qm.QM_EINVAL
+
+
 def test_workspace_covers_the_plain_call_and_the_pieces(qm):
     lib = qm.load_library()
     pool = ctypes.addressof(POOL)

@@ -22,6 +22,8 @@
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <utility>
+#include <vector>
 
 #include "qm_attention.h"
 
@@ -111,11 +113,15 @@ public:
     }
 
     // Workspace of launch_attention_shared for up to `max_batch` streams (about 20 MB more than plain attention needs).
-    // Allocates: call it before serving, not while a stream is being captured.
+    // Allocates: call it before serving, not while a stream is being captured.  A later call for more streams makes another
+    // workspace; the earlier one stays until this object goes, since captured launches keep its address.
     void reserve_shared_prefixes(int max_batch) {
-        shared_workspace_ = DeviceBuffer(static_cast<std::size_t>(qm_decode_shared_workspace_bytes(pool_, max_batch)));
-        check(qm_decode_workspace_init(shared_workspace_.pointer, static_cast<int64_t>(shared_workspace_.bytes), stream_),
-              "Talker shared-prefix workspace");
+        const std::size_t need = static_cast<std::size_t>(qm_decode_shared_workspace_bytes(pool_, max_batch));
+        if (shared_workspace_.pointer && shared_workspace_.bytes >= need) return;
+        DeviceBuffer made(need);
+        check(qm_decode_workspace_init(made.pointer, static_cast<int64_t>(made.bytes), stream_), "Talker shared-prefix workspace");
+        if (shared_workspace_.pointer) outgrown_workspaces_.push_back(std::move(shared_workspace_));
+        shared_workspace_ = std::move(made);
     }
 
     // Decode attention for groups of streams whose page tables begin with the same pages (one voice prompt behind many
@@ -261,6 +267,7 @@ private:
     cudaStream_t stream_;
     qm_kv_pool* pool_ = nullptr;
     DeviceBuffer rope_cos_, rope_sin_, workspace_, shared_workspace_;
+    std::vector<DeviceBuffer> outgrown_workspaces_;
 };
 
 }  // namespace qm

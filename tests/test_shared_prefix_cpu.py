@@ -1,8 +1,12 @@
 """Argument checks of the shared-prefix attention: every refusal comes back before any CUDA call."""
 import ctypes
+import shutil
+import subprocess
+from pathlib import Path
 
 import pytest
 
+ROOT = Path(__file__).resolve().parent.parent
 P = 0x10000
 
 
@@ -138,3 +142,15 @@ def test_a_workspace_that_could_not_be_prepared_is_not_kept(qm, monkeypatch):
     library.init = qm.QM_OK
     call()
     assert eng._shared_workspace is not None and library.prepared == 2
+
+
+def test_the_mirror_frees_no_workspace_that_a_launch_was_given(tmp_path):
+    """The C++ mirror with stand-ins for CUDA and the library, so that a workspace freed too early is seen on the CPU."""
+    binary = tmp_path / "shared_workspace_test"
+    toolkit = Path(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc").resolve().parent.parent
+    cmd = ["g++", "-std=c++17", "-O1", "-I", str(toolkit / "include"), "-I", str(ROOT / "include"), "-I",
+           str(ROOT / "qingming-qwen3-tts_b200" / "host"), str(ROOT / "tests" / "cpp" / "shared_workspace_test.cpp"), "-o", str(binary)]
+    built = subprocess.run(cmd, capture_output=True, text=True)
+    assert built.returncode == 0, built.stderr
+    ran = subprocess.run([str(binary)], capture_output=True, text=True, timeout=60)
+    assert ran.returncode == 0 and "SHARED_WORKSPACE_OK" in ran.stdout, ran.stdout + ran.stderr

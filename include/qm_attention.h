@@ -225,8 +225,10 @@ int32_t qm_decode_static_scratch_reset(qm_kv_pool* pool, void* stream);
 
 /* The same attention for streams that share a long prefix (many requests behind one voice prompt), the shared keys read
  * once per 64 streams instead of once per stream.  No counterpart in the reference (one stream; launch_attention with
- * query_length 1, 17.cu:17895).  Arguments and result are those of qm_decode_attention (a row may differ from it in
- * its last bf16 bits: the shared part runs on the tensor cores, its softmax weights rounded to bf16), and
+ * query_length 1, 17.cu:17895).  Arguments and result are those of qm_decode_attention, except that the softmax weights of
+ * the shared keys are rounded to bf16 for the product with V (it keeps them in fp32): an element may be further from the
+ * exact value by 2^-8 of sum_j p_j |v_j| over the shared keys; over many keys a row is off by 0.0023 of its norm where
+ * qm_decode_attention is by 0.0017, nearly all of it the result's own rounding.  And
  *   group_starts [groups + 1], shared_pages [groups]: streams group_starts[g] .. group_starts[g + 1] - 1 have the same first
  *     shared_pages[g] entries in their rows of page_table.  Nothing is copied or marked: those pages hold ordinary
  *     tokens, written by whichever stream was prefilled first, and a prefix that ends inside a page shares the pages in
@@ -235,7 +237,8 @@ int32_t qm_decode_static_scratch_reset(qm_kv_pool* pool, void* stream);
  * The entries need only agree among the group's streams that are at least shared_pages[g] * 64 keys long; a shorter
  * stream is attended on its own, as is one outside all groups.  group_starts that decrease or leave 0 .. batch are
  * forced into order and set QM_DEVSTAT_BAD_POS.
- * At most 256 streams and 256 groups per call (QM_ECAPACITY).  `workspace`: qm_decode_shared_workspace_bytes(pool, batch)
+ * At most 256 streams and 256 groups per call (QM_ECAPACITY).  It pays for groups of several streams with long prefixes:
+ * many groups of one or two streams are faster through qm_decode_attention.  `workspace`: qm_decode_shared_workspace_bytes(pool, batch)
  * bytes, 16-byte aligned, prepared once with qm_decode_workspace_init, and not shared by calls that overlap on the GPU
  * (it serves qm_decode_attention too, in turn).  The pool's device must be the current device.
  * Deterministic: the pieces depend on the lengths, the groups and the SM count, and are folded in order. */
@@ -438,9 +441,11 @@ int32_t qm_gate_up_swiglu_rows(qm_kv_pool* pool, const uint16_t* x, const uint16
 
 /* ---- the same projections with 8-bit integer operands ----
  * No counterpart in the reference (its projections, 17.cu:17646, :17691, :18020, are bf16).  Weights are int8 with one
- * fp32 scale per output channel, activations int8 with one fp32 scale per token row; the integer sums are exact:
+ * fp32 scale per output channel, activations int8 with one fp32 scale per token row:
  *   out[r][n] = bf16( float(sum_k x[r][k] * weight[n][k]) * x_scale[r] * weight_scale[n] + bias[n] + residual[r][n] )
- * with one rounding at the end.  qm_quantize_rows_int8 makes both operands (a weight matrix is a matrix of rows too).
+ * The integer sums are exact; their conversion to fp32 (which rounds past 2^24), the two products and the additions are
+ * fp32 operations, and the result is rounded to bf16.  qm_quantize_rows_int8 makes both operands (a weight matrix is a
+ * matrix of rows too).
  * Rows up to 2^31 - 256: up to 64 go through a split-K cluster kernel, more through persistent 128-row tiles.
  * in_features a multiple of 16, at most 65536; any out_features up to 2^31 - 256.  Tensors 16-byte aligned, x_scale 4-byte aligned;
  * bias and residual may be NULL.  The pool's device must be the current device. */

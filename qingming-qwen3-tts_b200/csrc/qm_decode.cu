@@ -158,8 +158,9 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) qm_decode_splitkv_kernel(co
 
     // A kernel that can allocate TMEM holds the SM's right to do so from its start, and no second CTA starts beside it
     // before it has given that up (measured: 148 CTAs at a time instead of 296, whether they allocate or not).  So every CTA
-    // allocates and relinquishes at once, and one without use for the columns frees them below.  The next launch is
-    // only let go after that: its CTAs may hold TMEM while they wait for this one.
+    // allocates and relinquishes at once, and one without use for the columns frees them below.  This variant lets no
+    // launch go early: the next one starts when it ends.  It is the fold, whose CTAs would come up packed on the SMs that
+    // finish first (20 us of fold instead of 7, measured).
     if constexpr (kShared) {
         if (warp == kPrefixTmemWarp) shared_prefix_tmem(smem_addr(smem + L::kFlagOff));
     } else {

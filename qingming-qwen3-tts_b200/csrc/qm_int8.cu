@@ -1,9 +1,10 @@
 // Projections with 8-bit integer operands: activations quantised per token row, weights per output channel.
 //
 //   s_x[r] = max_k |x[r][k]| / 127        q[r][k] = round(127 x[r][k] / max_k |x[r][k]|)      (ties to even)
-//   out[r][n] = (sum_k q[r][k] w[n][k]) * s_x[r] * s_w[n]  (+ bias[n]) (+ residual[r][n]), rounded to bf16 once
+//   out[r][n] = (sum_k q[r][k] w[n][k]) * s_x[r] * s_w[n]  (+ bias[n]) (+ residual[r][n])
 //
-// The integer sums are exact (kind::i8 accumulates in 32 bits; |sum| <= 128^2 K stays below 2^31 for K up to 65 536),
+// all of the second line after the sum in fp32, each operation rounded to it (the sum's conversion too, past 2^24), and the
+// result to bf16.  The integer sums are exact (kind::i8 accumulates in 32 bits; |sum| <= 128^2 K stays below 2^31 for K up to 65 536),
 // so neither the split of K over CTAs nor the order of the chunks can change a result.  No counterpart in the
 // reference, whose projections are bf16 only (launch_linear_m1 17.cu:17646, launch_qkv_m1 :17691,
 // launch_gate_up_swiglu_m1 :18020; the calls here have their shapes).  Against those, the weights are half the bytes,
@@ -217,7 +218,9 @@ __global__ void __launch_bounds__(kQuantWarps * 32, kNorm ? 3 : 4) qm_quantize_m
         if (lane + 32 * i < vectors)
             dst[lane + 32 * i] = quantize_eight<kNorm>(raw[i], kNorm ? __ldg(weights + lane + 32 * i) : none, r);
 }
-// Measured, us, a CTA per row / a warp per row: 2048 columns, 2048 rows 6.5 / 7.5, 4096 rows 12.1 / 8.7, 9923 rows 24.1 / 14.9.
+// Measured, us, a CTA per row / a warp per row: 2048 columns, 2048 rows 6.5 / 7.5, 4096 rows 12.1 / 8.7, 9923 rows 24.1 / 14.9;
+// other widths were not compared.  Wider rows have a CTA each whatever their number: 9923 rows of 6144 take 57 us, twice
+// what their bytes need.
 constexpr int kManyRows = 4096;
 
 // ---- shared by the two products -----------------------------------------------------------------------------------
@@ -484,9 +487,10 @@ qm_skinny_int8_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_co
 // Bound by operand bytes from the L2 (48 KB per 128 columns of K and SM; 670 cycles against 512 of the tensor pipe) and,
 // at small K, by the epilogue: 97 us = 2570 Tops for 9923 x 2048 x 6144, 187 us = 2940 Tops for 16384 x 4096 x 4096 (0.77
 // and 0.88 of twice the measured bf16 rate).  Four epilogue warps with scattered 16-byte stores and the column scales
-// read from global memory took 181 and 258 us.  Pairs of SMs on one tile of 256 x 256 (32 KB of operands instead of 48) gain
-// 1 to 4 % above 9000 rows, where the chip's power limit is near (114.7 instead of 97 us after 0.3 s of such launches), and lose 6 % between 1500 and 4000 rows to their longer
-// start and end; walking the tiles in groups of 4 to 16 rows of tiles changes neither.
+// read from global memory took 181 and 258 us.  Pairs of SMs on one tile of 256 x 256 (32 KB of operands instead of 48) were
+// measured and lose 6 % between 1500 and 4000 rows to their longer start and end; above 9000 rows the difference is within
+// what the chip's power limit does from run to run there (97 us, 115 after 0.3 s of such launches).  Walking the tiles in
+// groups of 4 to 16 rows of tiles changes neither.
 constexpr int kRowsThreads = 320;              // warps 0-7 epilogue, warp 8 MMA issue, warp 9 TMA loads
 constexpr int kRowsEpilogue = 256;
 constexpr int kStoreBytes = 32 * 32 * 2;       // 32 rows x 32 bf16 columns, 64-byte swizzle

@@ -21,10 +21,11 @@
 // same scan.  The few entries of that bin are gathered and put in order.  A bin with more than 512 entries
 // (many equal scores) is first cut down by digits of the entries' keys, which contain the index and therefore differ.  Where
 // top-k leaves few entries, they are gathered as a whole, and top-p, min-p and the draw need no sweep any more.
-// What bounds it: instructions (a weight is about 40, twelve of them in double precision; a top-p row of a large vocabulary
-// about 130 per score in all) and, for small rows, the steps' latency.  Measured: one row of 2048 with top-k 6.7 us, 64
-// rows of 2048 with everything 12 us, 32 rows of 131 072 fp32 45-52 us, 96 rows of 100 003 bf16 28 us without filters, 27 us
-// with top-k 50 (and top-p and min-p behind it), 18 us with min-p, 81 us with top-p 0.7 to 1.  Tried and slower, when that took
+// What bounds it: in many bf16 rows with top-p, instructions (a weight is about 40, twelve of them in double precision; 143 warp
+// instructions per 32 scores in all, at 2.1 of them per cycle); in few large fp32 rows and in small ones, the steps' latency (61
+// per 32 scores at 0.95 per cycle).  Measured: one row of 2048 with top-k 6.7 us, 64
+// rows of 2048 with everything 12 us, 32 rows of 131 072 fp32 44-45 us, 96 rows of 100 003 bf16 28 us without filters, 27 us
+// with top-k 50 (and top-p and min-p behind it), 18 us with min-p, 81-82 us with top-p 0.7 to 1.  Tried and slower, when that took
 // 92: the scores kept in shared memory (196 us; fewer CTAs fit), clusters of three with two CTAs on every SM (125 us), 512
 // threads per CTA (103 us, though 45 instead of 50 us at 131 072).
 #include <math_constants.h>

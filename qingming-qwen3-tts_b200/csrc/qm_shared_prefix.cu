@@ -10,10 +10,11 @@
 // tokens with up to 1024 of their own).  The second, below, folds a row's partial results: up to
 // a few dozen pieces of the shared part and one of its own, a CTA per pair of rows with its loads in flight together.
 //
-// Measured (8 KV heads): 64 streams behind 2048 tokens, up to 1024 of their own, 41-43 us (151 MB, 3.6 TB/s;
-// qm_decode_attention 100 us); 83 streams behind five prefixes of up to 4288 tokens, 44-48 us (184 us); 32 streams behind 32 768
-// tokens, 52-55 us (204 MB, 3.7 TB/s; 580 us).  What is left above the bytes' 22 to 31 us: about 3 us of plan, 4 us until the
-// first products, 6 us of fold, and CTAs with equal shares that end up to 10 us apart.
+// Measured (8 KV heads): 64 streams behind 2048 tokens, up to 1024 of their own, 42 us (151 MB, 3.6 TB/s;
+// qm_decode_attention 100 us); 83 streams behind five prefixes of up to 4288 tokens, 47-48 us (184 us); 32 streams behind 32 768
+// tokens, 52-53 us (204 MB, 3.9 TB/s; 581 us); four streams behind 1024 tokens 11 us (11 us).  What is left above the bytes' 22 to
+// 31 us: 1.3 to 2.1 us of plan, some 4 us until the first products, 7 to 9 us of fold and its launch, and CTAs with equal
+// shares that end up to 10 us apart.
 #include "qm_shared_prefix.cuh"
 
 namespace {

@@ -11,9 +11,10 @@
 #include "qm_tcgen05.cuh"
 
 constexpr int kSharedMaxBatch = 256;       // streams (and groups) per call
-// The costs that the cut goes by, in the time of a stream's own page.  Measured, us, at 0.85 / 0.95 / 1.05 per shared page: 64
-// streams behind 2048 tokens 42.8 / 43.0 / 44.2, 32 behind 32 768 tokens 53.2 / 54.4 / 56.2; at 3 instead of 1 per piece
-// 44.2 and 56.1.  Pieces of one page at least cost the first case 17.9 instead of 15.9 us of shared part alone.
+// The costs that the cut goes by, in the time of a stream's own page (measured with 8 KV heads only).  Measured, us, at
+// 0.85 / 0.95 / 1.05 per shared page: 64 streams behind 2048 tokens 42.8 / 43.0 / 44.2, 32 behind 32 768 tokens 53.2 / 54.4 /
+// 56.2; at 3 instead of 1 per piece 44.2 and 56.1.  Pieces of one page at least cost the first case 17.9 instead of 15.9 us of
+// shared part alone.
 constexpr float kSharedPageCost = 0.95f;   // a shared page (32 KB like an own one)
 constexpr float kSharedPieceCost = 1.0f;   // a piece, besides its pages
 constexpr int kOwnPartCost = 2;            // a stream's own part, besides its pages, per KV head (0 / 1 / 2: 83 streams behind five prefixes 50.7 / 48.0 / 47.5 us)
@@ -104,6 +105,10 @@ __device__ __forceinline__ int group_of_stream(const int* starts, int groups, in
 
 __device__ __forceinline__ int tiles_of(int streams) { return (streams + kStreamsPerTile - 1) / kStreamsPerTile; }
 
+// Small groups cost more than they save: a group is a 128-row tile however few its streams, and the search below walks
+// all groups before any CTA has work.  256 streams behind 512 shared tokens with 300 of their own take 110 us in 16 groups, 134
+// in 64, 176 in 128 and 243 in 256; qm_decode_attention over the same tables takes 129 to 132.
+//
 // Every CTA works the whole plan out for itself, from word `tid` of each array in thread `tid` (it may do so twice, from what
 // it read before and after the launch in front has written them).  first_page[s] = pages of stream s that are attended for
 // it.  `area`: SharedPlan::kBytes of shared memory.  All threads of the CTA; ends with a barrier.
@@ -251,9 +256,12 @@ __device__ __forceinline__ void publish_shared_plan(const SharedPlan& p, const S
 //
 // Per page: S = Q K^T (128 x 64, both operands by TMA, double-buffered in TMEM), a thread per row for the softmax, P
 // over S in bf16, O += P V with P as the TMEM operand.  P is rounded to bf16 (half a step is 2^-8 of each weight, and
-// the errors of many keys average out); the sum of exponentials is taken before that rounding, in fp32.  A row's O is
-// only rescaled when its maximum grew by more than 2^8 since the value in use.  Two CTAs fit an SM, one's softmax beside
-// the other's products.
+// the errors of many keys average out); the sum of exponentials is taken before that rounding, in fp32.  Against 64 bits a
+// context is off by 0.0022-0.0023 of its norm where fp32 weights (qm_decode_attention) leave 0.0017, nearly all of that the
+// rounding of the result.  P as a high and a low bf16 half, which has the 0.0017, was measured: 83 streams behind five
+// prefixes 47.8 -> 56.0 us, 32 behind 32 768 tokens 52.7 -> 61.4 us (one voice, 42 us, and four streams, 11 us, within
+// 0.6 us).  A row's O is only rescaled when its maximum grew by more than 2^8 since the value in use.  Two CTAs fit an SM,
+// one's softmax beside the other's products.
 constexpr int kPageBytes = kTileBytes;                 // K or V of one page and head
 constexpr int kPrefixQBytes = 128 * kHeadDim * 2;
 constexpr int kPageStages = 2;
